@@ -6,7 +6,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libq4gptq.so")
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 _lib = None
 
@@ -101,6 +101,31 @@ SIGNATURES["q4_gemm_grouped_bwd_dx_f16"] = (_i, [ctypes.POINTER(GemmLayer), _i, 
 MAX_GEMV_GROUP = 4
 SIGNATURES["q4_gemv_grouped_workspace_bytes"] = (_sz, [_i, _i])
 SIGNATURES["q4_gemv_grouped_f16"] = (_i, [ctypes.POINTER(GemvLayer), _i, _i, _i, _i, _i, _vp, _sz, _vp])
+
+
+class Kv4Cache(ctypes.Structure):
+    """q4_kv4_cache_t of include/q4_gptq.h."""
+    _fields_ = [("k_codes", _vp), ("v_codes", _vp), ("k_scales", _vp), ("v_scales", _vp), ("pages", _i), ("page", _i), ("heads", _i),
+                ("D", _i), ("group", _i)]
+
+
+class Kv4Batch(ctypes.Structure):
+    """q4_kv4_batch_t of include/q4_gptq.h."""
+    _fields_ = [("table", _vp), ("width", _i), ("lengths", _vp), ("starts", _vp), ("B", _i), ("T", _i)]
+
+
+class LoraRows(ctypes.Structure):
+    """q4_lora_rows_t of include/q4_gptq.h."""
+    _fields_ = [("a", _vp), ("b", _vp), ("scaling", _vp), ("y", _vp), ("N", _i)]
+
+
+_ll, _kv4 = ctypes.c_longlong, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Batch)]
+SIGNATURES["q4_kv4_append_f16"] = (_i, _kv4 + [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _vp, _i, _i, _i, _vp])
+SIGNATURES["q4_kv4_read_f16"] = (_i, _kv4 + [_vp, _vp, _vp])
+SIGNATURES["q4_kv4_attention_workspace_bytes"] = (_sz, _kv4 + [_i, _i, _i])
+SIGNATURES["q4_kv4_attention_f16"] = (_i, _kv4 + [_vp, _ll, _ll, _i, _f, _vp, _i, _i, _vp, _sz, _vp])
+SIGNATURES["q4_lora_rows_workspace_bytes"] = (_sz, [_i, _i, _i, _i])
+SIGNATURES["q4_lora_rows_f16"] = (_i, [ctypes.POINTER(LoraRows), _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp])
 
 
 class Q4Error(RuntimeError):

@@ -9,6 +9,7 @@
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <string>
@@ -688,6 +689,198 @@ void reset_workspaces() {
     for (auto& kv : g_mlp_buffers) kv.second.zero_();          // all zero = the state before a workspace's first use
 }
 
+// ---- serving many requests at once: the 4-bit key/value cache and the adapters of a batch's requests --------------------------
+// Workspaces come from the caching allocator call by call, not from this stream's buffers: a captured graph then owns its own, and two graphs
+// that were captured on one stream may be replayed side by side.
+
+// Inference only: a result would silently miss its gradient.
+void check_no_grad(const at::Tensor& t, const char* what) {
+    TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), what, " requires grad: this operator has no backward pass");
+}
+
+using Kv4Tensors = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+struct Kv4 {
+    q4_kv4_cache_t cache;
+    q4_kv4_batch_t batch;
+    c10::Device device;
+};
+
+Kv4 check_kv4(const Kv4Tensors& c, const at::Tensor& table, const at::Tensor& lengths, const c10::optional<at::Tensor>& starts, int64_t T) {
+    const at::Tensor &kc = std::get<0>(c), &vc = std::get<1>(c), &ks = std::get<2>(c), &vs = std::get<3>(c);
+    TORCH_CHECK_VALUE(kc.is_cuda(), "the cache must be on the GPU");
+    const auto dev = kc.device();
+    for (const at::Tensor* t : {&kc, &vc, &ks, &vs}) TORCH_CHECK_VALUE(t->is_contiguous() && t->device() == dev, "cache tensors must be contiguous and on one device");
+    TORCH_CHECK_VALUE(kc.scalar_type() == at::kInt && kc.dim() == 4 && vc.scalar_type() == at::kInt && vc.dim() == 5, "k_codes must be int32 [pages, heads, "
+                      "page, D/8] and v_codes int32 [pages, heads, page/4, D/8, 4]");
+    TORCH_CHECK_VALUE(ks.scalar_type() == at::kHalf && ks.dim() == 4 && vs.scalar_type() == at::kHalf && vs.sizes() == ks.sizes(),
+                      "k_scales and v_scales must be float16 [pages, heads, D/group, page]");
+    const int64_t P = kc.size(0), H = kc.size(1), page = kc.size(2), D = kc.size(3) * 8, NG = ks.size(2);
+    TORCH_CHECK_VALUE(P >= 1 && page >= 16 && page <= 1024 && page % 16 == 0, "pages must hold a multiple of 16 tokens, up to 1024; got ", page);
+    TORCH_CHECK_VALUE(D == 64 || D == 128, "heads must be 64 or 128 wide, got ", D);
+    TORCH_CHECK_VALUE(H >= 1 && H <= 4096, "the cache must hold 1..4096 heads, got ", H);
+    TORCH_CHECK_VALUE(vc.size(0) == P && vc.size(1) == H && vc.size(2) == page / 4 && vc.size(3) == D / 8 && vc.size(4) == 4 &&
+                      ks.size(0) == P && ks.size(1) == H && ks.size(3) == page && NG >= 1 && D % NG == 0 && D / NG >= 32,
+                      "the cache's tensors do not match each other");
+    TORCH_CHECK_VALUE(P < (1ll << 31) && P * H * NG * (page / 16) < (1ll << 31), "the cache is too large");
+    TORCH_CHECK_VALUE(table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous() && table.device() == dev,
+                      "page_table must be a contiguous int32 [B, pages of a sequence] tensor on the cache's device");
+    const int64_t B = table.size(0), width = table.size(1);
+    TORCH_CHECK_VALUE(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == B && lengths.is_contiguous() && lengths.device() == dev,
+                      "lengths must be a contiguous int32 [B] tensor on the cache's device");
+    const int* sp = nullptr;
+    if (starts.has_value()) {
+        TORCH_CHECK_VALUE(starts->scalar_type() == at::kInt && starts->dim() == 1 && starts->size(0) == B + 1 && starts->is_contiguous() &&
+                          starts->device() == dev, "starts must be a contiguous int32 [B + 1] tensor on the cache's device");
+        sp = starts->data_ptr<int>();
+    }
+    if (T > 0) {
+        TORCH_CHECK_VALUE(B >= 1 && width >= 1 && width * page <= (1 << 26), "page_table must cover 1 to 2^26 tokens of at least one sequence");
+        TORCH_CHECK_VALUE(sp || T % B == 0, "without starts every sequence has the same number of rows; got ", T, " rows of ", B, " sequences");
+        TORCH_CHECK_VALUE(T < (1ll << 31), "too many rows");
+    }
+    return Kv4{{kc.data_ptr<int>(), vc.data_ptr<int>(), ks.data_ptr(), vs.data_ptr(), (int)P, (int)page, (int)H, (int)D, (int)(D / NG)},
+               {table.data_ptr<int>(), (int)width, lengths.data_ptr<int>(), sp, (int)B, (int)T}, dev};
+}
+
+// fp16 [T, heads, D] whose dimensions lie side by side (token and head strides are free); `aligned`: in 16-byte pieces, copied if need be
+at::Tensor check_heads(const at::Tensor& t, int64_t T, int64_t D, const c10::Device& dev, bool aligned, const char* what) {
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kHalf && t.dim() == 3 && t.size(0) == T && t.size(2) == D && t.device() == dev, what,
+                      " must be float16 [rows, heads, ", D, "] on the cache's device");
+    check_no_grad(t, what);
+    if (t.size(0) == 0) return t;
+    const bool ok = t.stride(2) == 1 && t.stride(0) >= 0 && t.stride(1) >= 0;
+    if (!ok || (aligned && (t.stride(0) % 8 || t.stride(1) % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16))) return t.contiguous();
+    return t;
+}
+
+at::Tensor rows_out(const c10::optional<at::Tensor>& out, int64_t T, int64_t H, int64_t D, const at::Tensor& like, const char* what) {
+    if (!out.has_value()) return at::empty({T, H, D}, like.options());
+    TORCH_CHECK_VALUE(out->scalar_type() == at::kHalf && out->dim() == 3 && out->size(0) == T && out->size(1) == H && out->size(2) == D &&
+                      out->is_contiguous() && out->device() == like.device() && reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0, what,
+                      " must be a contiguous, 16-byte aligned float16 [", T, ", ", H, ", ", D, "] tensor on the cache's device");
+    return *out;
+}
+
+c10::optional<at::Tensor> kv4_append(const at::Tensor& k, const at::Tensor& v, const Kv4Tensors& cache, const at::Tensor& table,
+                                     const at::Tensor& lengths, const c10::optional<at::Tensor>& q, const c10::optional<at::Tensor>& rope,
+                                     bool interleaved, const c10::optional<at::Tensor>& starts, const c10::optional<at::Tensor>& q_out) {
+    TORCH_CHECK_VALUE(k.dim() == 3, "k must be float16 [rows, heads, D]");
+    const int64_t T = k.size(0);
+    const Kv4 c = check_kv4(cache, table, lengths, starts, T);
+    const at::Tensor k3 = check_heads(k, T, c.cache.D, c.device, false, "k"), v3 = check_heads(v, T, c.cache.D, c.device, false, "v");
+    TORCH_CHECK_VALUE(k.size(1) == c.cache.heads && v.size(1) == c.cache.heads, "k and v must have the cache's ", c.cache.heads, " heads");
+    at::Tensor q3, o;
+    if (q.has_value()) {
+        q3 = check_heads(*q, T, c.cache.D, c.device, false, "q");
+        o = rows_out(q_out, T, q->size(1), c.cache.D, *q, "q_out");
+    } else {
+        TORCH_CHECK_VALUE(!q_out.has_value(), "q_out needs q");
+    }
+    int64_t rows = 0, rot = 0;
+    if (rope.has_value()) {
+        TORCH_CHECK_VALUE(rope->scalar_type() == at::kFloat && rope->dim() == 3 && rope->size(2) == 2 && rope->is_contiguous() && rope->device() == c.device &&
+                          reinterpret_cast<uintptr_t>(rope->data_ptr()) % 16 == 0,
+                          "rope must be a contiguous float32 [positions, rotated/2, 2] tensor on the cache's device");
+        rows = rope->size(0);
+        rot = 2 * rope->size(1);
+        TORCH_CHECK_VALUE(rows >= 1 && rows < (1ll << 31) && rot >= 16 && rot <= c.cache.D && rot % 16 == 0,
+                          "rope must turn a multiple of 16 dimensions, at most the head's, at one position at least");
+    }
+    c10::optional<at::Tensor> result;
+    if (q.has_value()) result = o;
+    if (T == 0) return result;
+    Launch L(c.device);
+    const int rc = q4_kv4_append_f16(&c.cache, &c.batch, k3.data_ptr(), k3.stride(0), k3.stride(1), v3.data_ptr(), v3.stride(0), v3.stride(1),
+                                     q.has_value() ? q3.data_ptr() : nullptr, q.has_value() ? q3.stride(0) : 0, q.has_value() ? q3.stride(1) : 0,
+                                     q.has_value() ? o.data_ptr() : nullptr, q.has_value() ? (int)q3.size(1) : 0,
+                                     rot ? rope->data_ptr<float>() : nullptr, (int)rows, (int)rot, interleaved, L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_kv4_append_f16");
+    return result;
+}
+
+std::pair<at::Tensor, at::Tensor> kv4_read(const Kv4Tensors& cache, const at::Tensor& table, const at::Tensor& lengths, int64_t rows,
+                                           const c10::optional<at::Tensor>& starts) {
+    TORCH_CHECK_VALUE(rows >= 0, "the number of rows must not be negative");
+    const Kv4 c = check_kv4(cache, table, lengths, starts, rows);
+    const auto opts = std::get<2>(cache).options();
+    at::Tensor k = at::empty({rows, c.cache.heads, c.cache.D}, opts), v = at::empty({rows, c.cache.heads, c.cache.D}, opts);
+    if (rows == 0) return {k, v};
+    Launch L(c.device);
+    const int rc = q4_kv4_read_f16(&c.cache, &c.batch, k.data_ptr(), v.data_ptr(), L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_kv4_read_f16");
+    return {k, v};
+}
+
+at::Tensor kv4_attention(const at::Tensor& q, const Kv4Tensors& cache, const at::Tensor& table, const at::Tensor& lengths, double scale,
+                         const c10::optional<at::Tensor>& starts, c10::optional<int64_t> max_tokens, c10::optional<int64_t> max_length,
+                         const c10::optional<at::Tensor>& out) {
+    TORCH_CHECK_VALUE(q.dim() == 3, "q must be float16 [rows, heads, D]");
+    const int64_t T = q.size(0), H = q.size(1);
+    const Kv4 c = check_kv4(cache, table, lengths, starts, T);
+    const at::Tensor q3 = check_heads(q, T, c.cache.D, c.device, true, "q");
+    TORCH_CHECK_VALUE(H >= 1 && H % c.cache.heads == 0, "q must have a multiple of the cache's ", c.cache.heads, " heads, got ", H);
+    if (scale == 0.0) scale = 1.0 / std::sqrt((double)c.cache.D);
+    TORCH_CHECK_VALUE(scale > 0.0 && scale < 1e30, "scale must be positive and finite");
+    const at::Tensor o = rows_out(out, T, H, c.cache.D, q, "out");
+    if (T == 0) return o;
+    const int64_t all = (int64_t)c.batch.width * c.cache.page, most = starts.has_value() ? T : T / c.batch.B;
+    TORCH_CHECK_VALUE((!max_tokens.has_value() || *max_tokens >= 1) && (!max_length.has_value() || *max_length >= 1),
+                      "max_tokens and max_length must be at least 1");
+    const int mt = (int)std::min(most, max_tokens.value_or(most)), ml = (int)std::min(all, max_length.value_or(all));
+    Launch L(c.device);
+    const size_t need = q4_kv4_attention_workspace_bytes(&c.cache, &c.batch, (int)H, mt, ml);
+    at::Tensor ws;
+    if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+    const int rc = q4_kv4_attention_f16(&c.cache, &c.batch, q3.data_ptr(), q3.stride(0), q3.stride(1), (int)H, (float)scale, o.data_ptr(), mt, ml,
+                                        need ? ws.data_ptr() : nullptr, need, L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_kv4_attention_f16");
+    return o;
+}
+
+// (A [n, R, K], B [n, N, R], scaling [n], y [M, N]) of one layer
+using RowsSpec = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+void lora_rows(const at::Tensor& x, const at::Tensor& index, const std::vector<RowsSpec>& specs, int64_t per) {
+    const size_t count = specs.size();
+    TORCH_CHECK_VALUE(count >= 1 && count <= 4, "lora_rows takes 1..4 layers");
+    TORCH_CHECK_VALUE(x.is_cuda() && x.scalar_type() == at::kHalf && x.dim() == 2 && x.is_contiguous(), "x must be a contiguous float16 [M, K] CUDA tensor");
+    check_no_grad(x, "x");
+    const int64_t M = x.size(0), K = x.size(1);
+    TORCH_CHECK_VALUE(per >= 1 && index.scalar_type() == at::kInt && index.dim() == 1 && index.is_contiguous() && index.device() == x.device() &&
+                      index.size(0) == (M + per - 1) / per, "index must be a contiguous int32 tensor on x's device, one entry for each ", per, " rows");
+    q4_lora_rows_t probs[4];
+    int64_t n = 0, R = 0;
+    for (size_t i = 0; i < count; ++i) {
+        const at::Tensor &a = std::get<0>(specs[i]), &b = std::get<1>(specs[i]), &s = std::get<2>(specs[i]), &y = std::get<3>(specs[i]);
+        TORCH_CHECK_VALUE(a.scalar_type() == at::kHalf && a.dim() == 3 && a.size(2) == K && a.is_contiguous() && a.device() == x.device(),
+                          "A must be a contiguous float16 [n, R, ", K, "] tensor on x's device");
+        if (i == 0) { n = a.size(0); R = a.size(1); }
+        TORCH_CHECK_VALUE(a.size(0) == n && a.size(1) == R, "the layers of one call share the number of adapters and the rank");
+        TORCH_CHECK_VALUE(b.scalar_type() == at::kHalf && b.dim() == 3 && b.size(0) == n && b.size(2) == R && b.is_contiguous() && b.device() == x.device(),
+                          "B must be a contiguous float16 [n, N, R] tensor on x's device");
+        TORCH_CHECK_VALUE(s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == n && s.is_contiguous() && s.device() == x.device(),
+                          "scaling must be a contiguous float32 [n] tensor on x's device");
+        TORCH_CHECK_VALUE(y.scalar_type() == at::kHalf && y.dim() == 2 && y.size(0) == M && y.size(1) == b.size(1) && y.is_contiguous() &&
+                          y.device() == x.device(), "y must be a contiguous float16 [M, N] tensor on x's device");
+        for (const at::Tensor* t : {&a, &b, &y}) {
+            check_no_grad(*t, "a tensor of lora_rows");
+            TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "the tensors of lora_rows must be 16-byte aligned");
+        }
+        TORCH_CHECK_VALUE(y.size(1) >= 64 && y.size(1) % 64 == 0 && y.size(1) <= (1 << 23), "N must be a multiple of 64");
+        probs[i] = {a.data_ptr(), b.data_ptr(), s.data_ptr<float>(), y.data_ptr(), (int)y.size(1)};
+    }
+    TORCH_CHECK_VALUE(R >= 8 && R <= 64 && R % 8 == 0, "the rank must be a multiple of 8 in [8, 64], got ", R);
+    TORCH_CHECK_VALUE(K >= 32 && K % 32 == 0 && K <= (1 << 20) && M < (1 << 30), "K must be a multiple of 32");
+    TORCH_CHECK_VALUE(n < (1ll << 31) && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, "x must be 16-byte aligned");
+    if (M == 0 || n == 0) return;
+    Launch L(x.device());
+    const size_t need = q4_lora_rows_workspace_bytes((int)count, (int)M, (int)K, (int)R);
+    const at::Tensor ws = at::empty({(int64_t)need}, x.options().dtype(at::kByte));
+    const int rc = q4_lora_rows_f16(probs, (int)count, x.data_ptr(), index.data_ptr<int>(), (int)per, (int)M, (int)K, (int)R, (int)n, ws.data_ptr(), need,
+                                    L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_lora_rows_f16");
+}
+
 // True when the cached GEMV accumulators of every stream are all zero (synchronises; for tests and debugging).
 bool workspaces_are_zero() {
     std::lock_guard<std::mutex> lock(g_mutex);
@@ -744,6 +937,12 @@ PYBIND11_MODULE(_q4_host, m) {
           py::arg("out_shape") = py::none());
     m.def("silu_mul", &silu_mul, py::arg("gate"), py::arg("up"));
     m.def("silu_mul_bwd", &silu_mul_bwd, py::arg("dout"), py::arg("gate"), py::arg("up"));
+    m.def("kv4_append", &kv4_append, py::arg("k"), py::arg("v"), py::arg("cache"), py::arg("page_table"), py::arg("lengths"), py::arg("q") = py::none(),
+          py::arg("rope") = py::none(), py::arg("interleaved") = false, py::arg("starts") = py::none(), py::arg("q_out") = py::none());
+    m.def("kv4_read", &kv4_read, py::arg("cache"), py::arg("page_table"), py::arg("lengths"), py::arg("rows"), py::arg("starts") = py::none());
+    m.def("kv4_attention", &kv4_attention, py::arg("q"), py::arg("cache"), py::arg("page_table"), py::arg("lengths"), py::arg("scale") = 0.0,
+          py::arg("starts") = py::none(), py::arg("max_tokens") = py::none(), py::arg("max_length") = py::none(), py::arg("out") = py::none());
+    m.def("lora_rows", &lora_rows, py::arg("x"), py::arg("index"), py::arg("specs"), py::arg("per") = 1);
     m.def("mlp_decode_gave_up", &mlp_decode_gave_up);
     m.def("reset_workspaces", &reset_workspaces);
     m.def("workspaces_are_zero", &workspaces_are_zero);

@@ -366,6 +366,60 @@ typedef struct { const void *p, *in; float *out; int o_sr, o_sc, C; float alpha;
 Q4_API int q4_lora_grad_grouped_f32(const q4_lora_grad_t *probs, int n, int M, int R, void *workspace, size_t workspace_bytes,
                                     void *stream);
 
+/* ---- serving many requests at once ------------------------------------------------------------------------------------
+ * A paged cache of keys and values in 4 bits.  A value is code * scale: codes are 4-bit floats (1 sign, 2 exponent, 1 mantissa
+ * bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), scales fp16 = largest magnitude / 6 of `group` dimensions of one token and head.  With NG = D / group:
+ *   k_codes  int32 [pages, heads, page, D/8]       word kk*(D/32) + s (kk < 4) of a token: dimensions 32*s + 8*kk .. + 7, lowest nibble first
+ *   v_codes  int32 [pages, heads, page/4, D/8, 4]  word j of four tokens side by side; with H = D/16, nibble i + H*r is dimension 16*i + (D/8)*r + j
+ *   k_scales, v_scales  fp16 [pages, heads, NG, page]
+ * D 64 or 128; group 32, 64 or 128, at most D; page a multiple of 16 up to 1024; pages * heads * NG * page < 2^35.
+ * The reference keeps the host model's fp16 cache; no counterpart there. */
+typedef struct {
+    int32_t *k_codes, *v_codes;
+    void *k_scales, *v_scales;
+    int pages, page, heads, D, group;
+} q4_kv4_cache_t;
+/* The rows of a batch: rows starts[b] .. starts[b+1] - 1 (starts int32 [B+1], not falling; NULL: T / B each) are the last tokens of sequence b,
+ * which counts lengths[b] tokens, these included, on the pages table[b][0 .. width-1] (width * page <= 2^26).  All three are device memory and are
+ * read when the kernels run.  Whatever they hold, nothing outside the cache is touched: a row whose position is negative or behind the table, or whose
+ * page is not one of 0 .. pages - 1, has no place; rows outside starts[0] .. starts[B] - 1 belong to no sequence.  Sequences share pages only if none of
+ * the sharers appends to them. */
+typedef struct {
+    const int32_t *table;
+    int width;
+    const int32_t *lengths, *starts;
+    int B, T;
+} q4_kv4_batch_t;
+
+/* k, v fp16 (token and head strides in elements, dimensions side by side) go to the places of their rows; q (NULL: none) of q_heads heads comes out as
+ * q_out fp16 [T, q_heads, D].  The first `rot` dimensions (a multiple of 16, 0: none) of k and q are turned by pairs (x_i, x_{i+rot/2}), `interleaved`
+ * (x_{2i}, x_{2i+1}), with rope fp32 [rope_rows, rot/2, 2] = cosine and sine at the token's position; a position behind the table counts as no place.  A row
+ * without a place is not stored and its q_out is zero; a row of no sequence leaves everything as it was. */
+Q4_API int q4_kv4_append_f16(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, const void *k, long long k_t, long long k_h,
+                      const void *v, long long v_t, long long v_h, const void *q, long long q_t, long long q_h, void *q_out, int q_heads,
+                      const float *rope, int rope_rows, int rot, int interleaved, void *stream);
+
+/* k, v fp16 [T, heads, D] = what the cache holds at the places of the batch's rows (zero without a place). */
+Q4_API int q4_kv4_read_f16(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, void *k, void *v, void *stream);
+
+/* out fp16 [T, q_heads, D]: attention of each row over its sequence's keys at or before its own position, softmax(scale * q . k) v with
+ * q fp16 (strides as above, multiples of 8), q head h on key head h / (q_heads / heads).  A row that sees no key comes out as zero; keys without a
+ * place are not seen.  scale > 0.  `max_tokens` (rows of the longest sequence) and `max_length` (its tokens) size the launch; the result does not depend on
+ * their being right.  `workspace`: the bytes that the query gives for the same arguments (0: may be NULL), 256-byte aligned, contents irrelevant. */
+Q4_API size_t q4_kv4_attention_workspace_bytes(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, int q_heads, int max_tokens, int max_length);
+Q4_API int q4_kv4_attention_f16(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, const void *q, long long q_t, long long q_h, int q_heads,
+                         float scale, void *out, int max_tokens, int max_length, void *workspace, size_t workspace_bytes, void *stream);
+
+/* y_i fp16 [M, N_i] += scaling_i[a] * (x fp16 [M, K] @ A_i[a]^T) @ B_i[a]^T in place, a = index[m / per] (int32, device memory), for the
+ * `count` (1..4) layers that share x and the index: the adapters of the requests of a batch beside the products that they share (models.py:58-66 adds one
+ * adapter to all rows).  A_i fp16 [n, R, K], B_i fp16 [n, N_i, R], scaling_i fp32 [n]; R a multiple of 8 up to 64 (smaller adapters are filled up
+ * with zeros), K % 32 == 0, N_i % 64 == 0.  Rows whose index lies outside 0 .. n - 1 are left as they are.  The y_i must not overlap.
+ * `workspace`: q4_lora_rows_workspace_bytes bytes, 256-byte aligned, contents irrelevant. */
+typedef struct { const void *a, *b; const float *scaling; void *y; int N; } q4_lora_rows_t;
+Q4_API size_t q4_lora_rows_workspace_bytes(int count, int M, int K, int R);
+Q4_API int q4_lora_rows_f16(const q4_lora_rows_t *probs, int count, const void *x, const int32_t *index, int per, int M, int K, int R, int n,
+                     void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
