@@ -102,8 +102,8 @@ __device__ __forceinline__ half2_t kv4_pair(uint32_t w) {
     return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, SEL);
 }
 __device__ __forceinline__ half8_t kv4_word(uint32_t w) {
-    const half2_t a = kv4_pair<0>(w), b = kv4_pair<1>(w), c = kv4_pair<2>(w), d = kv4_pair<3>(w);
-    return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    const uint4_t x = {as_u32(kv4_pair<0>(w)), as_u32(kv4_pair<1>(w)), as_u32(kv4_pair<2>(w)), as_u32(kv4_pair<3>(w))};
+    return __builtin_bit_cast(half8_t, x);
 }
 // codes of eight values, to nearest, ties to the even code, beyond 6 to 6
 __device__ __forceinline__ uint32_t kv4_codes(const float* y) {

@@ -7,17 +7,48 @@
 // fp16 is the only one before the output's.
 #include "q4_kv4.hpp"
 #include <algorithm>
+#include <type_traits>
 
 namespace q4 {
 
 // Probabilities are formed as 2^10 * exp(s - m): times a value's scale they then stay clear of fp16's subnormals down to 1e-7 of the
 // largest for scales of 0.1, and below its largest number for scales up to 32; for larger scales the maximum is raised.
 constexpr float kBoost = 10.0f, kMostScale = 32.0f;
+constexpr uint32_t kMostScaleBits = 0x5000u;          // 32 in fp16
 
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Maximum over the four lanes r, r + 16, r + 32, r + 48: rows of 16 lanes change places in registers.  (The results are copied out of their vector
+// first: a bit cast straight from its second element reads the first.)
+__device__ __forceinline__ float max_of_rows(float x) {
+    uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    u = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+    const auto b = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
+__device__ __forceinline__ float max_of_halves(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    return fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+}
+
+typedef float float2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t rounded_pair(float a, float b) { return as_u32(__builtin_convertvector(float2_t{a, b}, half2_t)); }
+
+__device__ __forceinline__ bool finite_bits(half_t x) { return (__builtin_bit_cast(uint16_t, x) & 0x7C00u) != 0x7C00u; }
+
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, a), __builtin_bit_cast(ushort2_t, b)));
 }
 
 // ---- up to 16 rows a workgroup ------------------------------------------------------------------
@@ -30,14 +61,7 @@ __device__ __forceinline__ void wave_lds_fence() {
 //                  4 x 4 words of keys 16*kk ..: neighbouring keys' nibbles side by side by two operations per four pairs
 // so no operand passes through LDS, and maximum, sum and rescaling belong to the lane.
 template <int D, int NG>
-struct Kv4Tile {
-    uint32_t k[4][D / 32];
-    uint4_t v[4];
-    uint4_t sc;               // eight scales: lane (kv, group, eighth of the tile)
-};
-
-template <int D, int NG>
-__global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
+__global__ __launch_bounds__(256, 3) void kv4_attn_rows_kernel(Kv4Attn a) {
     constexpr int S = D / 32, H = D / 16, SG = S / NG, HG = H / NG, W = D / 8;
     __shared__ __attribute__((aligned(16))) half_t scales[4][2][NG][64];
     __shared__ __attribute__((aligned(16))) float red[4][16][D + 4];
@@ -92,79 +116,84 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
             w.y = head * NG * p16 + off;
             return w;
         };
-        auto load = [&](Kv4Tile<D, NG>& x, uint2_t at) {
-            const uint32_t kr = (uint32_t)__shfl((int)at.x, r >> 2) & 0x7FFFFFFFu, vr = (uint32_t)__shfl((int)at.x, kk) & 0x7FFFFFFFu;
+        // Registers of one tile: the keys' are requested again as soon as the scores are formed, the values' as soon as they are multiplied.
+        uint32_t xk[4][S];
+        uint4_t xv[4], xs = {0u, 0u, 0u, 0u};                              // xs: eight scales, lane = (keys or values, group, eighth of the tile)
+        auto load_keys = [&](uint2_t at) {
+            const uint32_t kr = (uint32_t)__shfl((int)at.x, r >> 2) & 0x7FFFFFFFu;
             const uint32_t* kp = a.c.kc + (size_t)kr * (16 * W) + (r & 3) * W + kk * S;
-            const uint32_t* vp = a.c.vc + (size_t)vr * (16 * W) + (r % W) * 4;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                if constexpr (S == 4) *reinterpret_cast<uint4_t*>(x.k[u]) = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(kp + u * 4 * W));
-                else *reinterpret_cast<uint2_t*>(x.k[u]) = __builtin_nontemporal_load(reinterpret_cast<const uint2_t*>(kp + u * 4 * W));
+                if constexpr (S == 4) *reinterpret_cast<uint4_t*>(xk[u]) = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(kp + u * 4 * W));
+                else *reinterpret_cast<uint2_t*>(xk[u]) = __builtin_nontemporal_load(reinterpret_cast<const uint2_t*>(kp + u * 4 * W));
             }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) x.v[u] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(vp + u * 4 * W));
             const int piece = lane & 7, g = (lane >> 3) % NG;
             const uint32_t sr = (uint32_t)__shfl((int)at.y, piece >> 1);
             if (lane < 16 * NG)
-                x.sc = *reinterpret_cast<const uint4_t*>((lane < 8 * NG ? a.c.ks : a.c.vs) + ((size_t)sr + g * p16) * 16 + 8 * (piece & 1));
+                xs = *reinterpret_cast<const uint4_t*>((lane < 8 * NG ? a.c.ks : a.c.vs) + ((size_t)sr + g * p16) * 16 + 8 * (piece & 1));
         };
-        auto compute = [&](const Kv4Tile<D, NG>& x, uint2_t at, int tile) {
-            if (lane < 16 * NG) *reinterpret_cast<uint4_t*>(&scales[wave][0][0][0] + 8 * lane) = x.sc;
+        auto load_values = [&](uint2_t at) {
+            const uint32_t vr = (uint32_t)__shfl((int)at.x, kk) & 0x7FFFFFFFu;
+            const uint32_t* vp = a.c.vc + (size_t)vr * (16 * W) + (r % W) * 4;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) xv[u] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(vp + u * 4 * W));
+        };
+        float s[16];
+        auto scores = [&] {
+            if (lane < 16 * NG) *reinterpret_cast<uint4_t*>(&scales[wave][0][0][0] + 8 * lane) = xs;
             wave_lds_fence();
-            float s[16];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 float4_t acc[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) acc[u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int st = g * SG; st < (g + 1) * SG; ++st)
+                for (int st = g * SG; st < (g + 1) * SG; ++st) {
+                    __builtin_amdgcn_sched_barrier(0);                     // or all operands are built first, in registers that are not there
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
-                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_word(x.k[u][st]), qf[st], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_word(xk[u][st]), qf[st], acc[u], 0, 0, 0);
+                }
                 const half8_t k0 = *reinterpret_cast<const half8_t*>(&scales[wave][0][g][16 * kk]);
                 const half8_t k1 = *reinterpret_cast<const half8_t*>(&scales[wave][0][g][16 * kk + 8]);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const float ks = (float)(e < 8 ? k0[e & 7] : k1[e & 7]);
                     s[e] = g == 0 ? acc[e >> 2][e & 3] * ks : fmaf(acc[e >> 2][e & 3], ks, s[e]);
+                    asm volatile("" : "+v"(s[e]));                         // here, not where it is used: one group's sums at a time
                 }
             }
-            half8_t sv[NG][2];
+        };
+        auto weigh = [&](bool masked, int seen, bool unusual) {
+            if (masked) {                                                  // whatever a place that is not seen holds, it counts nothing
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int v = 0; v < 2; ++v) sv[g][v] = *reinterpret_cast<const half8_t*>(&scales[wave][1][g][16 * kk + 8 * v]);
-            __builtin_amdgcn_wave_barrier();
-            const bool bad = (uint32_t)__shfl((int)at.x, kk) >> 31;
-            if (tile * 64 + 64 > kmin || __any(bad)) {                     // whatever a place that is not seen holds, it counts nothing
-                const int seen = bad ? 0 : limit - (tile * 64 + 16 * kk);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[e] = e < seen ? s[e] : -INFINITY;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) sv[g][e >> 3][e & 7] = e < seen ? sv[g][e >> 3][e & 7] : (half_t)0.f;
-                }
+                for (int e = 0; e < 16; ++e) s[e] = e < seen ? s[e] : -INFINITY;
             }
             float mx = s[0];
 #pragma unroll
             for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-            half8_t big8 = sv[0][0];
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int v = 0; v < 2; ++v) big8 = __builtin_elementwise_max(big8, sv[g][v]);
-            half_t bigh = big8[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) bigh = __builtin_elementwise_max(bigh, big8[e]);
-            float big = (float)bigh;
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            float mn = mx * a.scale;
-            if (__any(big > kMostScale)) {
-                big = fmaxf(big, __shfl_xor(big, 16));
-                big = fmaxf(big, __shfl_xor(big, 32));
-                mn += log2f(fmaxf(big, kMostScale) / kMostScale);
+            float mn = max_of_rows(mx) * a.scale;
+            if (unusual) {
+                // Scales above kMostScale raise the maximum.  One that is no number makes the row none that sees it; it is zero for the others, whose
+                // weight of nothing times it would not be nothing.
+                float big = kMostScale;
+#pragma unroll 1
+                for (int i = 0; i < 16 * NG; ++i) {
+                    const half_t x = scales[wave][1][i >> 4][16 * kk + (i & 15)];
+                    if ((i & 15) < seen) {
+                        if (finite_bits(x)) big = fmaxf(big, (float)x);
+                        else l = NAN;
+                    }
+                }
+                mn += log2f(max_of_rows(big) / kMostScale);
+                wave_lds_fence();
+                if (lane >= 8 * NG && lane < 16 * NG) {
+                    half_t* x = &scales[wave][0][0][0] + 8 * lane;
+#pragma unroll 1
+                    for (int e = 0; e < 8; ++e)
+                        if (!finite_bits(x[e])) x[e] = (half_t)0.f;
+                }
+                wave_lds_fence();
             }
             mn = fmaxf(m, mn);
             const float base = mn == -INFINITY ? 0.f : mn;
@@ -175,18 +204,18 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
                 for (int i = 0; i < H; ++i) o[i] *= f;
                 m = mn;
             }
-            float p[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, kBoost - base));
-                l += p[e];
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale, kBoost - base));
+                l += s[e];
             }
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
+                __builtin_amdgcn_sched_barrier(0);
                 uint32_t lo[4], hi[4];                                     // even and odd nibbles of two keys side by side
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const uint4_t w = x.v[2 * v + (c >> 1)];
+                    const uint4_t w = xv[2 * v + (c >> 1)];
                     uint32_t wa = c & 1 ? w.z : w.x, wb = c & 1 ? w.w : w.y;
                     if constexpr (D == 64) { wa >>= 16 * (r >> 3); wb >>= 16 * (r >> 3); }
                     lo[c] = (wa & 0x0F0F0F0Fu) | ((wb << 4) & 0xF0F0F0F0u);
@@ -194,40 +223,51 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
                 }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    half8_t pb;
+                    if (NG > 1) __builtin_amdgcn_sched_barrier(0);
+                    const half8_t sv = *reinterpret_cast<const half8_t*>(&scales[wave][1][g][16 * kk + 8 * v]);
+                    uint4_t pw;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) pb[e] = (half_t)(p[8 * v + e] * (float)sv[g][v][e]);
+                    for (int e = 0; e < 4; ++e)
+                        pw[e] = rounded_pair(fmaf(s[8 * v + 2 * e], (float)sv[2 * e], 0.f), fmaf(s[8 * v + 2 * e + 1], (float)sv[2 * e + 1], 0.f));
+                    const half8_t pb = __builtin_bit_cast(half8_t, pw);
 #pragma unroll
                     for (int i = g * HG; i < (g + 1) * HG; ++i) {
-                        half8_t va;
+                        uint4_t vw;
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             const uint32_t w = i & 1 ? hi[c] : lo[c];
-                            const half2_t d = i / 2 == 0 ? kv4_pair<0>(w) : i / 2 == 1 ? kv4_pair<1>(w) : i / 2 == 2 ? kv4_pair<2>(w) : kv4_pair<3>(w);
-                            va[2 * c] = d[0];
-                            va[2 * c + 1] = d[1];
+                            vw[c] = as_u32(i / 2 == 0 ? kv4_pair<0>(w) : i / 2 == 1 ? kv4_pair<1>(w) : i / 2 == 2 ? kv4_pair<2>(w) : kv4_pair<3>(w));
                         }
-                        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, o[i], 0, 0, 0);
+                        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, vw), pb, o[i], 0, 0, 0);
                     }
                 }
             }
         };
 
-        // tiles wave, wave + 4, ... of the share; while one is worked on, the next one's codes and the page entries of the one behind it are on their way
-        Kv4Tile<D, NG> xa, xb;
+        // tiles wave, wave + 4, ... of the share; the page entries are looked up one tile further ahead
         int t = split * per + wave;
-        uint2_t pa = {0u, 0u}, pb = {0u, 0u};
-        if (t < t_end) { pa = look_up(t); load(xa, pa); pb = look_up(t + 4); }
-        for (; t < t_end; t += 8) {
-            uint2_t pc = {0u, 0u};
-            if (t + 4 < t_end) { load(xb, pb); pc = look_up(t + 8); }
-            compute(xa, pa, t);
-            if (t + 4 >= t_end) break;
-            pa = pc;
-            uint2_t pd = {0u, 0u};
-            if (t + 8 < t_end) { load(xa, pa); pd = look_up(t + 12); }
-            compute(xb, pb, t + 4);
-            pb = pd;
+        uint2_t at = {0u, 0u}, next = {0u, 0u};
+        if (t < t_end) {
+            at = look_up(t);
+            next = look_up(t + 4);
+            load_keys(at);
+            load_values(at);
+        }
+        while (t < t_end) {
+            const bool more = t + 4 < t_end;
+            scores();
+            // whether a value's scale is above kMostScale or no number, seen or not, by its bits, where the tile's scales lie eight in a lane
+            uint32_t most = pk_max_u16(pk_max_u16(xs.x, xs.y), pk_max_u16(xs.z, xs.w));
+            most = lane >= 8 * NG && lane < 16 * NG ? max(most >> 16, most & 0xFFFFu) : 0u;
+            const bool bad = (uint32_t)__shfl((int)at.x, kk) >> 31;
+            at = next;
+            if (more) {
+                next = look_up(t + 8);
+                load_keys(at);
+            }
+            weigh(t * 64 + 64 > kmin || __any(bad), bad ? 0 : limit - (t * 64 + 16 * kk), __any(most > kMostScaleBits));
+            if (more) load_values(at);
+            t += 4;
         }
 
         l += __shfl_xor(l, 16);
@@ -260,7 +300,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
             if (a.nsplit == 1) {
                 half4_t y;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = (half_t)(top == -INFINITY ? 0.f : v[e] / sum);
+                for (int e = 0; e < 4; ++e) y[e] = (half_t)(sum == 0.f ? 0.f : v[e] / sum);
                 *reinterpret_cast<half4_t*>(a.out + at * D + d) = y;
             } else {
                 const size_t all = (size_t)a.p.T * a.hq;
@@ -270,6 +310,304 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4Attn a) {
                     ml[0] = top;
                     ml[1] = sum;
                 }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- prompts: 128 rows a workgroup -----------------------------------------------------------------
+// Four wavefronts of 32 rows on the same tiles of 64 keys.  The workgroup turns a tile's codes into fp16 values (one rounding each, of code * scale) in LDS, in
+// the order in which v_mfma_f32_32x32x16_f16 takes them: pieces of 16 bytes, lane after lane, so that neither side meets a bank conflict.  Two tiles: the next one
+// is written, and the one behind it requested, while one is multiplied; one barrier a tile.  As above S^T = K Q^T and O^T = V^T P^T, lane (r, h) holding row r:
+//   keys' piece (kb, st, lane): key 32*kb + r, dimensions 16*st + 8*h .. + 7
+//   values' piece (kb, p, db, lane): dimension 32*db + r of keys 32*kb + 16*p + 4*h + (0..3) and + 8, the keys of the scores in that lane's registers 8*p .. + 7
+// The maximum that weights refer to is raised only when a score lies 2^kSlack above it: weights then stay below 2^15.
+constexpr float kSlack = 5.0f;
+constexpr int kPromptRows = 128;
+
+template <int D>
+struct Kv4Staged {
+    uint4_t k[2 * D / 16 * 64], v[4 * D / 32 * 64];
+};
+
+template <int D, int NG>
+__global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
+    constexpr int S = D / 32, ST = D / 16, DB = D / 32, W = D / 8, SG = S / NG, H = D / 16, HG = H / NG, NV = D / 16;   // NV: nibbles of a word a thread takes
+    __shared__ __attribute__((aligned(16))) Kv4Staged<D> tiles_lds[2];
+    __shared__ int poison;                                                 // first key seen whose values are no numbers
+    __shared__ int there[2][4];                                            // whether the tile's runs of 16 keys lie on pages of the cache
+    const int lane = threadIdx.x & 63, r = lane & 31, h32 = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int id = blockIdx.x;
+    const int h = id % a.c.heads;                                          // workgroups on one head's keys lie on one chiplet where heads are a multiple of 8
+    id /= a.c.heads;
+    const int split = id % a.nsplit;
+    id /= a.nsplit;
+    const int b = id % a.p.B, block0 = a.blocks - 1 - id / a.p.B;          // the rows with the most keys first
+    const int first = a.p.starts ? a.p.starts[b] : b * (a.p.T / a.p.B);
+    const int n = min((a.p.starts ? a.p.starts[b + 1] : (b + 1) * (a.p.T / a.p.B)) - first, a.p.T);
+    const int len = a.p.lengths[b], cap = a.p.width * a.c.page, p16 = a.c.page / 16;
+    const int* table = a.p.table + (size_t)b * a.p.width;
+    const int rows = n * a.share;
+
+    for (int row0 = block0 * kPromptRows; row0 < rows; row0 += a.blocks * kPromptRows) {
+        const int row = row0 + 32 * wave + r;
+        const int tok = first + row / a.share, qh = h * a.share + row % a.share;
+        const bool live = row < rows && tok >= 0 && tok < a.p.T;
+        const int limit = live ? max(0, min(len - n + row / a.share + 1, cap)) : 0;
+        // 0 .. kmin - 1 are seen by all rows of this wavefront, kend by any of the workgroup's
+        const int kmin = max(0, min(len - n + (row0 + 32 * wave) / a.share + 1, cap));
+        const int kend = max(0, min(len - n + min(row0 + kPromptRows - 1, rows - 1) / a.share + 1, cap));
+        const int tiles = (kend + 63) / 64, per = (tiles + a.nsplit - 1) / a.nsplit;
+        const int t0 = split * per, t_end = min(t0 + per, tiles);
+        if (threadIdx.x == 0) poison = 0x7FFFFFFF;
+
+        half8_t qf[ST];
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+            qf[s] = half8_t{};
+            if (live) qf[s] = *reinterpret_cast<const half8_t*>(a.q + tok * a.q_t + qh * a.q_h + 16 * s + 8 * h32);
+        }
+        float16_t o[DB];
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+        float m = -INFINITY, l = 0.f;
+
+        // This thread's part of a tile: a quarter of the words of key 16*wave + c, and word c of the four keys of block 4*wave + kk: all in run `wave`.
+        // Two tiles are on their way, and the page of the one behind them.
+        const int c = lane & 15, kk = lane >> 4;
+        struct Raw {
+            uint32_t k[S];
+            uint4_t v;
+            half_t ks[NG];
+            half4_t vs[NG];
+            bool have;
+        } raw[2];
+        int page = -1;                                                     // of the next tile to be requested
+        auto page_of = [&](int tile) {                                     // uniform
+            const int run = tile * 4 + wave;
+            return tile < t_end && run * 16 < kend ? table[a.page_magic ? (int)__umulhi((uint32_t)run, a.page_magic) : run] : -1;
+        };
+        auto request = [&](Raw& x, int tile) {
+            const int run = tile * 4 + wave;
+            const int idx = a.page_magic ? (int)__umulhi((uint32_t)run, a.page_magic) : run;
+            x.have = page >= 0 && page < a.c.pages;
+            const uint32_t head = (uint32_t)(x.have ? page : 0) * a.c.heads + h, off = x.have ? run - idx * p16 : 0;
+            page = page_of(tile + 1);
+            const uint32_t* kp = a.c.kc + (size_t)(head * p16 + off) * (16 * W) + c * W + kk * S;
+            if constexpr (S == 4) *reinterpret_cast<uint4_t*>(x.k) = *reinterpret_cast<const uint4_t*>(kp);
+            else *reinterpret_cast<uint2_t*>(x.k) = *reinterpret_cast<const uint2_t*>(kp);
+            x.v = *reinterpret_cast<const uint4_t*>(a.c.vc + (size_t)(head * p16 + off) * (16 * W) + (kk * W + c % W) * 4);
+            const size_t sc = ((size_t)head * NG * p16 + off) * 16;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                x.ks[g] = a.c.ks[sc + (size_t)g * a.c.page + c];
+                x.vs[g] = *reinterpret_cast<const half4_t*>(a.c.vs + sc + (size_t)g * a.c.page + 4 * kk);
+            }
+        };
+        // What no row of the workgroup sees is nothing, and a value's scale that is no number makes the rows none that see it.
+        auto look = [&](Raw& x, int buf, int tile) {
+            const int key = tile * 64 + 16 * wave;
+            if (lane == 0) there[buf][wave] = x.have || key >= kend;
+            const int ks_in = x.have ? kend - key - c : 0, vs_in = x.have ? kend - key - 4 * kk : 0;
+            int strange = 0x7FFFFFFF;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                if (ks_in <= 0) x.ks[g] = (half_t)0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool finite = finite_bits(x.vs[g][e]);
+                    if (e < vs_in && !finite) strange = min(strange, key + 4 * kk + e);
+                    if (e >= vs_in || !finite) x.vs[g][e] = (half_t)0.f;
+                }
+            }
+            if (__any(strange != 0x7FFFFFFF)) atomicMin(&poison, strange);
+        };
+        const int kb_w = wave >> 1;                                        // the half of a tile that this wavefront's keys lie in
+        auto stage_keys = [&](const Raw& x, int buf) {
+            const int kr = 16 * (wave & 1) + c;
+#pragma unroll
+            for (int s = 0; s < S; ++s) {                                  // dimensions 32*s + 8*kk .. + 7
+                const half2_t f = {x.ks[s / SG], x.ks[s / SG]};
+                const uint4_t y = {as_u32(kv4_pair<0>(x.k[s]) * f), as_u32(kv4_pair<1>(x.k[s]) * f), as_u32(kv4_pair<2>(x.k[s]) * f),
+                                   as_u32(kv4_pair<3>(x.k[s]) * f)};
+                tiles_lds[buf].k[(kb_w * ST + 2 * s + (kk >> 1)) * 64 + 32 * (kk & 1) + kr] = y;
+            }
+        };
+        auto stage_values = [&](const Raw& x, int buf) {
+            // block 4*wave + kk of the tile: keys 4*kk .. of this half of its 32; piece p = wave & 1, h = kk & 1, half of it kk >> 1
+            uint32_t wd[4] = {x.v.x, x.v.y, x.v.z, x.v.w};
+            if constexpr (D == 64) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) wd[e] >>= 16 * (c >> 3);
+            }
+            uint32_t pr[2][2];                                             // [pair of keys][even, odd nibbles]
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                pr[q][0] = (wd[2 * q] & 0x0F0F0F0Fu) | ((wd[2 * q + 1] << 4) & 0xF0F0F0F0u);
+                pr[q][1] = ((wd[2 * q] >> 4) & 0x0F0F0F0Fu) | (wd[2 * q + 1] & 0xF0F0F0F0u);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {                                 // dimension 16*i + c
+                uint2_t y;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const uint32_t w = pr[q][i & 1];
+                    const half2_t f = {x.vs[i / HG][2 * q], x.vs[i / HG][2 * q + 1]};
+                    const half2_t d = i / 2 == 0 ? kv4_pair<0>(w) : i / 2 == 1 ? kv4_pair<1>(w) : i / 2 == 2 ? kv4_pair<2>(w) : kv4_pair<3>(w);
+                    y[q] = as_u32(d * f);
+                }
+                uint4_t* at = &tiles_lds[buf].v[((kb_w * 2 + (wave & 1)) * DB + i / 2) * 64 + 32 * (kk & 1) + 16 * (i & 1) + c];
+                reinterpret_cast<uint2_t*>(at)[kk >> 1] = y;
+            }
+        };
+        // Tile t from half BUF, while t + 1 goes to the other one; behind the last tile that is written once more, for nobody.
+        auto step = [&](auto half, int t) {
+            constexpr int BUF = decltype(half)::value;
+            const Kv4Staged<D>& x = tiles_lds[BUF];
+            Raw& next = raw[BUF ^ 1];
+            const int th[4] = {there[BUF][0], there[BUF][1], there[BUF][2], there[BUF][3]};
+            look(next, BUF ^ 1, t + 1);
+            float16_t s[2];
+            __builtin_amdgcn_sched_barrier(0);
+            stage_keys(next, BUF ^ 1);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+                for (int st = 0; st < ST; ++st)
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, x.k[(kb * ST + st) * 64 + lane]), qf[st], s[kb], 0, 0, 0);
+            }
+            // the conversion of the next keys goes between the products, operands three products ahead
+            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * ST; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+                __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (t * 64 + 64 > kmin || !(th[0] & th[1] & th[2] & th[3])) {  // register e of block kb: key 32*kb + 8*(e/4) + 4*h32 + e%4
+                const int seen = limit - (t * 64 + 4 * h32);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int until = th[2 * kb + (e >> 3)] ? seen : 0;
+                        s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) < until ? s[kb][e] : -INFINITY;
+                    }
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int e = 1; e < 32; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
+            mx = max_of_halves(mx) * a.scale;
+            if (__any(mx > m + kSlack)) {
+                const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < DB; ++i) o[i] *= f;
+                m = mn;
+            }
+            const float base = kBoost - (m == -INFINITY ? 0.f : m);
+            uint4_t pw[4];
+            auto weights = [&](int kb) {
+                float part = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], a.scale, base));
+                    part += s[kb][e];
+                }
+                l += part;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pw[2 * kb + (e >> 2)][e & 3] = rounded_pair(s[kb][2 * e], s[kb][2 * e + 1]);
+            };
+            auto values = [&](int kb) {
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int i = 0; i < DB; ++i)
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, x.v[((kb * 2 + p) * DB + i) * 64 + lane]),
+                                                                      __builtin_bit_cast(half8_t, pw[2 * kb + p]), o[i], 0, 0, 0);
+            };
+            weights(0);
+            __builtin_amdgcn_sched_barrier(0);
+            values(0);
+            weights(1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * DB; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            values(1);
+            stage_values(next, BUF ^ 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * DB; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            request(next, t + 3);
+            __syncthreads();
+        };
+
+        __syncthreads();
+        if (t0 < t_end) {
+            page = page_of(t0);
+            request(raw[0], t0);
+            request(raw[1], t0 + 1);
+            look(raw[0], 0, t0);
+            stage_keys(raw[0], 0);
+            stage_values(raw[0], 0);
+            request(raw[0], t0 + 2);
+        }
+        __syncthreads();
+        for (int t = t0; t < t_end; t += 2) {
+            step(std::integral_constant<int, 0>{}, t);
+            if (t + 1 >= t_end) break;
+            step(std::integral_constant<int, 1>{}, t + 1);
+        }
+        if (limit > poison) l = NAN;
+        {
+            const uint32_t lb = __builtin_bit_cast(uint32_t, l);
+            const auto x = __builtin_amdgcn_permlane32_swap(lb, lb, false, false);
+            const uint32_t x0 = x[0], x1 = x[1];
+            l = __builtin_bit_cast(float, x0) + __builtin_bit_cast(float, x1);
+        }
+        if (live) {                                                        // o[i][e]: dimension 32*i + 8*(e/4) + 4*h32 + e%4
+            const size_t at = (size_t)tok * a.hq + qh, all = (size_t)a.p.T * a.hq;
+            const float f = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int d = 32 * i + 8 * q + 4 * h32;
+                    if (a.nsplit == 1) {
+                        half4_t y;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = (half_t)(o[i][4 * q + e] * f);
+                        *reinterpret_cast<half4_t*>(a.out + at * D + d) = y;
+                    } else {
+                        float4_t y;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = o[i][4 * q + e];
+                        *reinterpret_cast<float4_t*>(a.part + (split * all + at) * D + d) = y;
+                    }
+                }
+            if (a.nsplit > 1 && h32 == 0) {
+                float* ml = a.part + a.nsplit * all * D + (split * all + at) * 2;
+                ml[0] = m;
+                ml[1] = l;
             }
         }
         __syncthreads();
@@ -320,21 +658,24 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4Attn a) {
         float y = 0.f;
 #pragma unroll
         for (int s = 0; s < PER; ++s) y += acc[s][threadIdx.x];
-        a.out[row * D + threadIdx.x] = (half_t)(top == -INFINITY ? 0.f : y / sum);
+        a.out[row * D + threadIdx.x] = (half_t)(sum == 0.f ? 0.f : y / sum);
     }
 }
 
 // ---- plan ----------------------------------------------------------------------------------------
-struct Kv4AttnPlan { int blocks, nsplit; };
+struct Kv4AttnPlan { bool prompt; int blocks, nsplit; };
 
-// Row blocks of 16 for the longest run of new tokens; the keys in shares until about four workgroups stand for every compute unit, a share
-// of 256 keys (a tile per wavefront) at least.
+// Above 64 rows a key head and sequence the prompt kernel, below it 16 rows a workgroup.  The keys are split until about four (prompts: two)
+// workgroups stand for every compute unit, a share of 256 keys (a tile per wavefront) at least.
 inline Kv4AttnPlan plan_kv4_attn(int B, int heads, int share, int max_tokens, int max_length) {
     Kv4AttnPlan p;
-    p.blocks = (int)(((long)max_tokens * share + 15) / 16);
-    const long groups = (long)B * heads * p.blocks;
-    const long most = std::max(1, (max_length + 255) / 256);
-    p.nsplit = (int)std::max(1l, std::min({most, (1024 + groups - 1) / groups, 256l}));
+    const long rows = (long)max_tokens * share;
+    p.prompt = rows > 64;
+    const int per = p.prompt ? kPromptRows : 16;
+    p.blocks = (int)((rows + per - 1) / per);
+    const long groups = (long)B * heads * p.blocks, wanted = p.prompt ? 512 : 1024;
+    const long most = std::max(1l, (max_length + 255l) / 256);
+    p.nsplit = (int)std::max(1l, std::min({most, (wanted + groups - 1) / groups, 256l}));
     return p;
 }
 
@@ -346,9 +687,10 @@ size_t q4_kv4_attn_workspace(int B, int heads, int D, int share, int T, int max_
 }
 
 template <int D, int NG>
-static void launch_rows(const q4::Kv4Attn& a, hipStream_t stream) {
+static void launch_attn(const q4::Kv4Attn& a, bool prompt, hipStream_t stream) {
     const dim3 grid((unsigned)((long)a.p.B * a.blocks * a.c.heads * a.nsplit));
-    hipLaunchKernelGGL((q4::kv4_attn_rows_kernel<D, NG>), grid, dim3(256), 0, stream, a);
+    if (prompt) hipLaunchKernelGGL((q4::kv4_attn_prompt_kernel<D, NG>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((q4::kv4_attn_rows_kernel<D, NG>), grid, dim3(256), 0, stream, a);
     if (a.nsplit > 1)
         hipLaunchKernelGGL((q4::kv4_attn_join_kernel<D>), dim3((unsigned)((long)a.p.T * a.hq)), dim3(256), 0, stream, a);
 }
@@ -360,11 +702,11 @@ int q4_launch_kv4_attn(q4::Kv4Attn& a, int D, int group, int max_tokens, int max
     const uint32_t p16 = a.c.page / 16;
     a.page_magic = p16 == 1 ? 0u : (uint32_t)(((1ull << 32) + p16 - 1) / p16);
     switch (D / group + (D == 64 ? 8 : 0)) {
-        case 1: launch_rows<128, 1>(a, stream); break;
-        case 2: launch_rows<128, 2>(a, stream); break;
-        case 4: launch_rows<128, 4>(a, stream); break;
-        case 9: launch_rows<64, 1>(a, stream); break;
-        default: launch_rows<64, 2>(a, stream); break;
+        case 1: launch_attn<128, 1>(a, p.prompt, stream); break;
+        case 2: launch_attn<128, 2>(a, p.prompt, stream); break;
+        case 4: launch_attn<128, 4>(a, p.prompt, stream); break;
+        case 9: launch_attn<64, 1>(a, p.prompt, stream); break;
+        default: launch_attn<64, 2>(a, p.prompt, stream); break;
     }
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }

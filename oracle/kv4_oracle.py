@@ -107,14 +107,16 @@ def places(table, lengths, starts, rows, pages, page):
     return out
 
 
-def attention(q, cache, table, lengths, starts, scale):
+def attention(q, cache, table, lengths, starts, scale, rounded=False):
     """(out, tol) float64 [T, Hq, D] for float16 q: the formula, and how far a kernel may be off that forms scores and sums in float32, rounds the weights
-    (times 2^10 and the value's scale) to fp16 once and the output once.  Rows of no sequence: NaN.
+    (times 2^10 and the value's scale) to fp16 once and the output once; `rounded`: that also rounds every key and value, code * scale, to fp16 once
+    (the weights then without the value's scale).  Rows of no sequence: NaN.
 
     Terms of tol: half a step of the output, 2^-11 |o| (2^-25 where it is subnormal); half a step of every weight, 2^-11 sum p |v|, or 2^-25 * 6 in units of
     2^10 for subnormal ones (fewer where scales above 32 raise the maximum); twice (numerator and denominator) the relative error of a weight, exp of a score that is off by (D + 8) float32 half steps of
     sum |q k| and whose product with scale and difference to the maximum (at most 2 max |s|) round, and two steps of the exponential; the sums over L keys, of at most
-    L / 32 + 64 additions one after the other."""
+    L / 32 + 64 additions one after the other.  `rounded`: a score is off by 2^-11 sum |q k| more (2^-25 sum |q| for subnormal keys), the values by 2^-11 sum p |v|
+    and 2^-25."""
     pages, heads, page = cache[0].shape[:3]
     T, Hq, D = q.shape
     share, u = Hq // heads, 2.0 ** -24
@@ -142,7 +144,11 @@ def attention(q, cache, table, lengths, starts, scale):
                     p /= p.sum()
                     o, pv = p @ v, p @ np.abs(v)
                     eps = mag * (D + 8) * u + 4 * np.abs(s).max() * u + 4 * u
+                    more, unit = 0.0, 6 * big
+                    if rounded:
+                        eps += mag * 2.0 ** -11 + scale * np.abs(x).sum() * 2.0 ** -25
+                        more, unit = 2.0 ** -11 * pv + 2.0 ** -25, max(unit, np.abs(v).max())
                     L = len(seen)
                     out[t, qh] = o
-                    tol[t, qh] = (2.0 ** -11 * np.abs(o) + 2.0 ** -25 + (2.0 ** -11 + 2 * eps + (L / 32 + 64) * 2 * u) * pv + L * 6 * big * 2.0 ** -35)
+                    tol[t, qh] = (2.0 ** -11 * np.abs(o) + 2.0 ** -25 + (2.0 ** -11 + np.expm1(2 * eps) + (L / 32 + 64) * 2 * u) * pv + L * unit * 2.0 ** -35 + more)
     return out, tol

@@ -38,6 +38,9 @@ def _filled(o, lengths, heads, D, group, page, rng, spread=1.0):
     return cache, table
 
 
+PROMPT_ROWS = 64            # more rows a key head and sequence (tokens times the heads that share it) go to the kernel that rounds keys and values too
+
+
 def _check(got, want, tol, what=""):
     got = got.float().cpu().numpy().astype(np.float64)
     mine = ~np.isnan(want)
@@ -73,7 +76,7 @@ def test_attention_matches_float64(heads, share, D, group, page, lengths, new):
     rng = np.random.default_rng(sum(lengths) + new + D + group)
     cache, table = _filled(o, lengths, heads, D, group, page, rng)
     q = (rng.standard_normal((len(lengths) * new, heads * share, D)) * 2).astype(np.float16)
-    want, tol = o.attention(q, cache, table, np.array(lengths), None, 1 / math.sqrt(D))
+    want, tol = o.attention(q, cache, table, np.array(lengths), None, 1 / math.sqrt(D), new * share > PROMPT_ROWS)
     dev, tb, ln = [_cuda(x) for x in cache], _cuda(table), torch.tensor(lengths, dtype=torch.int32).cuda()
     got = quant_hip.kv4_attention(_cuda(q), tuple(dev), tb, ln)
     _check(got, want, tol)
@@ -97,7 +100,7 @@ def test_attention_of_ragged_rows_views_and_padding(new):
     T = int(starts[-1]) + 5
     qkv = rng.standard_normal((T, heads * share * D + 24)).astype(np.float16)
     q = _cuda(qkv)[:, 8:8 + heads * share * D].unflatten(-1, (heads * share, D))
-    want, tol = o.attention(q.cpu().numpy(), cache, table, np.array(lengths), starts, 0.11)
+    want, tol = o.attention(q.cpu().numpy(), cache, table, np.array(lengths), starts, 0.11, True)
     out = torch.full((T, heads * share, D), 7.0, dtype=torch.float16, device="cuda")
     args = (tuple(_cuda(x) for x in cache), _cuda(table), torch.tensor(lengths, dtype=torch.int32).cuda())
     for bounds in ({}, {"max_tokens": max(new), "max_length": max(lengths)}, {"max_tokens": max(new), "max_length": 5000}):
@@ -115,7 +118,7 @@ def test_attention_of_ragged_rows_views_and_padding(new):
     _check(got, want, tol, "heads first")
 
 
-@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("new", [1, 20, 60])
 def test_attention_with_bad_pages_and_poison_in_places_that_are_not_seen(new):
     """Pages that do not exist hide their keys; later tokens of the same prompt may hold infinities and NaN; a length beyond the table ends with it."""
     import torch
@@ -128,7 +131,7 @@ def test_attention_with_bad_pages_and_poison_in_places_that_are_not_seen(new):
     table[0, 2], table[0, 5], table[1, 0], table[2, :] = cache[0].shape[0], -7, 2 ** 30, -1
     claimed = np.array([150, 90, 64 + 10 ** 6], np.int32)
     q = rng.standard_normal((3 * new, heads * share, D)).astype(np.float16)
-    want, tol = o.attention(q, cache, table, claimed, None, 0.1)
+    want, tol = o.attention(q, cache, table, claimed, None, 0.1, new * share > PROMPT_ROWS)
     args = (tuple(_cuda(x) for x in cache), _cuda(table), _cuda(claimed))
     _check(quant_hip.kv4_attention(_cuda(q), *args, scale=0.1), want, tol)
     assert np.all(want[2 * new:] == 0)
@@ -149,16 +152,16 @@ def test_attention_with_large_and_small_scales():
     from oracle import kv4_oracle as o
     heads, D, group, page = 1, 128, 32, 32
     rng = np.random.default_rng(3)
-    for spread in (1e-4, 3000.0):
+    for spread, n in ((1e-4, 1), (3000.0, 1), (1e-4, 70), (3000.0, 70)):
         lengths = [333]
         cache, table = _filled(o, lengths, heads, D, group, page, rng, spread)
         cache[2][:] = np.where(np.isnan(cache[2]), cache[2], np.float16(0.2))          # keys of ordinary size
         if spread > 1:
             cache[3][table[0, 3], 0, 1] = np.float16(10000.0)
-        q = (rng.standard_normal((1, 1, D)) * 20).astype(np.float16)
-        want, tol = o.attention(q, cache, table, np.array(lengths), None, 1 / math.sqrt(D))
+        q = (rng.standard_normal((n, 1, D)) * 20).astype(np.float16)
+        want, tol = o.attention(q, cache, table, np.array(lengths), None, 1 / math.sqrt(D), n > PROMPT_ROWS)
         got = quant_hip.kv4_attention(_cuda(q), tuple(_cuda(x) for x in cache), _cuda(table), torch.tensor(lengths, dtype=torch.int32).cuda())
-        _check(got, want, tol, spread)
+        _check(got, want, tol, (spread, n))
 
 
 APPEND = [
