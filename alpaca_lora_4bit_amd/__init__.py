@@ -7,6 +7,7 @@ Sub-modules keep the reference's names so its callers read unchanged:
     models               Linear4bitLt, GPTQLoraModel
     monkeypatch.peft_tuners_lora_monkey_patch   replace_peft_model_with_int4_lora_model
     arg_parser, Finetune4bConfig, train_data, gradient_checkpointing   what the finetune script imports
+    kv4_cache            the 4-bit paged key/value cache of many requests (no counterpart in the reference)
     finetune, inference  the reference's two top-level scripts as runnable modules (python -m ...)
 
 `install_as_alpaca_lora_4bit()` registers these modules under the reference's package name so
@@ -22,7 +23,7 @@ __version__ = "0.1.0"
 
 _ALIASED = ("autograd_4bit", "matmul_utils_4bit", "quant_hip", "models", "amp_wrapper", "model_attn_mlp_patch",
             "loaders", "arg_parser", "Finetune4bConfig", "train_data", "gradient_checkpointing", "monkeypatch",
-            "monkeypatch.peft_tuners_lora_monkey_patch")
+            "monkeypatch.peft_tuners_lora_monkey_patch", "kv4_cache")
 
 
 def install_as_alpaca_lora_4bit(name: str = "alpaca_lora_4bit") -> None:

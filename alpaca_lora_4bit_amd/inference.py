@@ -14,8 +14,13 @@ runs the MLP decode step (gate, up, silu * up, down) as one launch, adapters inc
 and `--hip_graph` captures the one-token step once as a HIP graph and replays it per token, which removes the host
 time of the ~1000 small launches a decoder step consists of; the choice of the next token (argmax with `--greedy`,
 otherwise the reference's sampling settings) runs eagerly between two replays.
+
+`--requests FILE` answers many prompts together, each with the adapter of its own choice: a JSON object per line,
+`{"prompt": ..., "lora": directory}` ("lora" may be left out).  Their keys and values are held in 4 bits in a paged cache
+(kv4_cache.py) and their adapters beside each other (models.AdapterBank); see `generate_batch`.
 """
 import argparse
+import json
 import time
 
 import torch
@@ -39,6 +44,7 @@ def _parse(argv):
     p.add_argument("--greedy", action="store_true", help="argmax decoding instead of sampling")
     p.add_argument("--fuse", action="store_true", help="one launch for q+k+v and one for gate+up")
     p.add_argument("--hip_graph", action="store_true", help="decode with the token step replayed as a HIP graph")
+    p.add_argument("--requests", default=None, help="file with a JSON object per line, {\"prompt\": ..., \"lora\": directory}: answer them as one batch")
     return p.parse_args(argv)
 
 
@@ -140,8 +146,200 @@ def greedy_generate_graph(model, input_ids, max_new_tokens, eos_token_id=None):
     return generate_graph(model, input_ids, max_new_tokens, eos_token_id=eos_token_id)
 
 
+class _BatchModel:
+    """A LLaMA's blocks over rows of many sequences: the modules of the loaded model do the products and norms, the keys and values go through
+    the 4-bit paged cache and every row's own adapter is added to the products."""
+
+    def __init__(self, model, cache, bank, positions):
+        from .kv4_cache import rope_table
+        cfg = model.config
+        self.model, self.cache, self.bank = model, cache, bank
+        self.heads, self.kv_heads, self.head_dim = _attention_shape(cfg)
+        self.rope = rope_table(model.model.rotary_emb, positions, cache.device)
+
+    def _add(self, x, index, *pairs):
+        if self.bank is not None and index is not None:
+            self.bank.apply(x, index, pairs)
+
+    def _mlp(self, mlp, x, index):
+        if index is None or self.bank is None or not self.bank.holds(mlp.gate_proj, mlp.up_proj, mlp.down_proj):
+            return mlp(x)
+        gate, up = mlp.gate_proj(x), mlp.up_proj(x)
+        self._add(x, index, (mlp.gate_proj, gate), (mlp.up_proj, up))
+        act = (mlp.act_fn(gate) * up).contiguous()
+        out = mlp.down_proj(act)
+        self._add(act, index, (mlp.down_proj, out))
+        return out
+
+    def __call__(self, ids, table, lengths, starts, index, max_tokens, max_length, wanted=None):
+        """Logits [rows, vocabulary] of the rows `ids` (`wanted`: of these rows only); see quant_hip.kv4_attention for the batch's tensors."""
+        from . import quant_hip
+        net = self.model.model
+        h = net.embed_tokens(ids)
+        for block, layer in zip(net.layers, self.cache.layers):
+            attn = block.self_attn
+            x = block.input_layernorm(h).contiguous()
+            q, k, v = attn.q_proj(x), attn.k_proj(x), attn.v_proj(x)
+            self._add(x, index, (attn.q_proj, q), (attn.k_proj, k), (attn.v_proj, v))
+            k, v = (t.view(-1, self.kv_heads, self.head_dim) for t in (k, v))
+            q = quant_hip.kv4_append(k, v, layer, table, lengths, q=q.view(-1, self.heads, self.head_dim), rope=self.rope, starts=starts)
+            o = quant_hip.kv4_attention(q, layer, table, lengths, starts=starts, max_tokens=max_tokens, max_length=max_length)
+            o = o.view(-1, self.heads * self.head_dim)
+            out = attn.o_proj(o)
+            self._add(o, index, (attn.o_proj, out))
+            h = h + out
+            h = h + self._mlp(block.mlp, block.post_attention_layernorm(h).contiguous(), index)
+        if wanted is not None:
+            h = h[wanted]
+        return self.model.lm_head(net.norm(h))
+
+
+def _attention_shape(cfg):
+    if getattr(cfg, "model_type", None) != "llama":
+        raise ValueError(f"batches of requests are built for LLaMA models, not for {getattr(cfg, 'model_type', None)!r}")
+    heads = cfg.num_attention_heads
+    return heads, getattr(cfg, "num_key_value_heads", None) or heads, getattr(cfg, "head_dim", None) or cfg.hidden_size // heads
+
+
+def generate_batch(model, prompts, max_new_tokens, bank=None, adapters=None, eos_token_id=None, sampling=None, use_graph=True,
+                   page=64, group=32, prefill_rows=8192):
+    """Continues many prompts together.  `prompts`: 1-D id tensors, of any lengths; `adapters`: for each of them the number of its adapter in
+    `bank` (a models.AdapterBank), or -1.  The prompts run without padding, their rows one after another, in parts of at most `prefill_rows`
+    rows; then every step answers one token of every request, its forward captured once as a HIP graph (`use_graph`) as in
+    `generate_graph`.  Keys and values are held in 4 bits with a scale per `group` dimensions, in pages of `page` tokens.  Returns a list of id
+    tensors, prompt and answer, each ended by `eos_token_id` or after `max_new_tokens`."""
+    from .kv4_cache import PagedKv4Cache
+    count = len(prompts)
+    if count == 0 or max_new_tokens < 1:
+        return [p.clone() for p in prompts]
+    if any(p.dim() != 1 or p.numel() == 0 for p in prompts):
+        raise ValueError("prompts must be 1-D tensors of at least one id")
+    if (bank is None) != (adapters is None) or (adapters is not None and len(adapters) != count):
+        raise ValueError("`bank` and `adapters` (one number for each prompt) go together")
+    if adapters is not None and any(not -1 <= a < bank.count for a in adapters):
+        raise ValueError(f"adapters must be -1 .. {bank.count - 1}")
+    if prefill_rows < 1:
+        raise ValueError("prefill_rows must be positive")
+    heads, kv_heads, head_dim = _attention_shape(model.config)
+    dev = prompts[0].device
+    totals = [p.numel() + max_new_tokens for p in prompts]
+    longest = max(totals)
+    pages = sum(-(-t // page) for t in totals)
+    pick = _token_picker(sampling)
+    ints = dict(dtype=torch.int32)
+    with torch.no_grad():
+        cache = PagedKv4Cache(len(model.model.layers), kv_heads, head_dim, pages, page, group, dev)
+        run = _BatchModel(model, cache, bank, longest)
+        handles = [cache.open(t) for t in totals]
+        index = None if adapters is None else torch.tensor(list(adapters), **ints).to(dev)
+
+        # the prompts, in parts of at most prefill_rows rows: each part is runs of tokens of some requests
+        parts, part, room = [], [], prefill_rows
+        for b, p in enumerate(prompts):
+            done = 0
+            while done < p.numel():
+                take = min(room, p.numel() - done)
+                part.append((b, done, done + take))
+                done += take
+                room -= take
+                if room == 0:
+                    parts.append(part)
+                    part, room = [], prefill_rows
+        if part:
+            parts.append(part)
+        first = [None] * count
+        for part in parts:
+            rows = [stop - start for _, start, stop in part]
+            starts = [0]
+            for r in rows:
+                starts.append(starts[-1] + r)
+            ends = [(b, starts[i + 1] - 1) for i, (b, _, stop) in enumerate(part) if stop == prompts[b].numel()]
+            logits = run(torch.cat([prompts[b][start:stop] for b, start, stop in part]), cache.table([handles[b] for b, _, _ in part]),
+                         torch.tensor([stop for _, _, stop in part], **ints).to(dev), torch.tensor(starts, **ints).to(dev),
+                         None if index is None else torch.repeat_interleave(index[[b for b, _, _ in part]], torch.tensor(rows, device=dev)),
+                         max(rows), max(stop for _, _, stop in part), torch.tensor([row for _, row in ends], dtype=torch.long, device=dev))
+            for (b, _), line in zip(ends, logits):
+                first[b] = line
+
+        table = cache.table(handles)
+        lengths = torch.tensor([p.numel() for p in prompts], **ints).to(dev)
+        tokens = torch.zeros(count, dtype=prompts[0].dtype, device=dev)
+        alive = torch.ones(count, **ints).to(dev)
+        ids = list(prompts)
+        going = [True] * count
+
+        def advance(logits):
+            """The next token of every request; True when all of them have ended.  An ended request keeps its row, with a length of zero: nothing
+            of it is stored and its attention reads nothing."""
+            if sampling is None:
+                nxt = logits.argmax(-1)
+            else:
+                nxt = torch.cat([pick(ids[b][None], logits[b][None])[0] if going[b] else tokens[b:b + 1] for b in range(count)])
+            nxt = nxt.to(tokens.dtype)
+            for b in range(count):
+                if going[b]:
+                    ids[b] = torch.cat([ids[b], nxt[b:b + 1]])
+            tokens.copy_(nxt)
+            if eos_token_id is not None:
+                for b, t in enumerate(nxt.tolist()):
+                    if going[b] and t == eos_token_id:
+                        going[b] = False
+                        alive[b] = 0
+                        lengths[b] = 0
+            return not any(going)
+
+        def step():
+            lengths.add_(alive)
+            return run(tokens, table, lengths, None, index, 1, longest)
+
+        left = max_new_tokens - 1
+        done = advance(torch.stack(first))
+        graph = None
+        while left and not done:
+            if graph is not None:
+                graph.replay()
+            elif left == max_new_tokens - 1 and use_graph and left > 1:
+                # one eager step on a side stream first: every lazy allocation and per-layer check happens there
+                side = torch.cuda.Stream()
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    logits = step()
+                torch.cuda.current_stream().wait_stream(side)
+            elif use_graph:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    logits = step()
+                graph.replay()
+            else:
+                logits = step()
+            left -= 1
+            done = advance(logits)
+        return ids
+
+
+def _answer_requests(model, tokenizer, args):
+    """--requests: (texts, seconds)."""
+    from . import models
+    with open(args.requests) as fh:
+        requests = [json.loads(line) for line in fh if line.strip()]
+    dirs = sorted({r["lora"] for r in requests if r.get("lora")})
+    bank = models.AdapterBank(model, dirs) if dirs else None
+    adapters = [dirs.index(r["lora"]) if r.get("lora") else -1 for r in requests] if dirs else None
+    prompts = [tokenizer(r["prompt"], return_tensors="pt", add_special_tokens=False)["input_ids"][0].cuda() for r in requests]
+    sampling = None if args.greedy else {k: SAMPLING[k] for k in ("repetition_penalty", "temperature", "top_k", "top_p")}
+    start = time.time()
+    sequences = generate_batch(model, prompts, args.max_new_tokens, bank, adapters, eos_token_id=getattr(tokenizer, "eos_token_id", None),
+                               sampling=sampling, use_graph=args.hip_graph)
+    texts = [tokenizer.decode(s.tolist()) for s in sequences]
+    seconds = time.time() - start
+    for text in texts:
+        print(text)
+    print(seconds)
+    return texts, seconds
+
+
 def main(argv=None):
-    """Returns (text, seconds)."""
+    """Returns (text, seconds); with --requests (texts, seconds)."""
     args = _parse(argv)
     from . import models
     from .amp_wrapper import AMPWrapper
@@ -162,6 +360,9 @@ def main(argv=None):
     if args.fuse:
         from .model_attn_mlp_patch import make_fused_mlp, make_quant_attn
         print("Fused", make_quant_attn(model), "attention blocks and", make_fused_mlp(model), "MLP blocks")
+
+    if args.requests is not None:
+        return _answer_requests(model, tokenizer, args)
 
     print("Apply AMP Wrapper ...")
     AMPWrapper(model).apply_generate()

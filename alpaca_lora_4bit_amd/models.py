@@ -322,3 +322,75 @@ def inject_lora_layers(model, target_modules=("q_proj", "v_proj"), r=8, lora_alp
                 GPTQLoraModel._replace_module(parent, child_name, new, child)
                 replaced[f"{parent_name}.{child_name}" if parent_name else child_name] = new
     return replaced
+
+
+class AdapterBank:
+    """The adapters of many requests for one model, each layer's side by side, so that one batch can hold requests with different adapters (or
+    none): `apply` adds every row's own adapter to the products that all rows share (quant_hip.lora_rows), where the reference holds one adapter for
+    the whole batch (models.py:51-69).  Matrices are held in fp16, the type the products run in; ranks are padded with zeros to the largest one,
+    rounded up to a multiple of 8 (up to 64)."""
+
+    def __init__(self, model, adapters, device="cuda"):
+        """adapters: directories as `finetune` or peft write them (adapter_config.json and the tensors), or (state dict, scaling) pairs.  Number i of
+        the list is adapter i of the index that `apply` takes."""
+        import json
+        import os
+        from .model_attn_mlp_patch import _read_adapter_state
+        modules = dict(model.named_modules())
+        parts, scalings = {}, []                             # module -> {(adapter, 'lora_A' | 'lora_B'): tensor}
+        for number, source in enumerate(adapters):
+            if isinstance(source, (str, os.PathLike)):
+                with open(os.path.join(source, "adapter_config.json")) as fh:
+                    cfg = json.load(fh)
+                state, scaling = _read_adapter_state(source), cfg["lora_alpha"] / cfg["r"]
+            else:
+                state, scaling = source
+            scalings.append(float(scaling))
+            for key, tensor in state.items():
+                path = key[len("base_model.model."):] if key.startswith("base_model.model.") else key
+                name, dot, part = path.partition(".lora_")
+                layer = modules.get(name)
+                if not dot or part[:1] not in ("A", "B"):
+                    raise ValueError(f"adapter {number}: {key} is not a matrix of a LoRA layer")
+                if layer is None or not hasattr(layer, "in_features"):
+                    raise ValueError(f"adapter {number} names {name}, which the model does not have")
+                want = layer.in_features if part[0] == "A" else layer.out_features
+                if tensor.dim() != 2 or tensor.shape[1 if part[0] == "A" else 0] != want:
+                    raise ValueError(f"adapter {number}: {key} is {tuple(tensor.shape)}, the layer has {layer.in_features} -> {layer.out_features}")
+                parts.setdefault(layer, {})[(number, part[0])] = tensor
+        self.count = len(scalings)
+        self._layers = {}
+        for layer, found in parts.items():
+            rank = 0
+            for (number, part), tensor in found.items():
+                other = found.get((number, "B" if part == "A" else "A"))
+                r = tensor.shape[0 if part == "A" else 1]
+                if other is None or other.shape[1 if part == "A" else 0] != r:
+                    raise ValueError(f"adapter {number}: lora_A and lora_B of a layer do not belong together")
+                rank = max(rank, r)
+            if rank < 1 or rank > 64:
+                raise ValueError(f"the rank of an adapter must be 1 to 64, not {rank}")
+            rank = -(-rank // 8) * 8
+            a = torch.zeros((self.count, rank, layer.in_features), dtype=torch.float16, device=device)
+            b = torch.zeros((self.count, layer.out_features, rank), dtype=torch.float16, device=device)
+            for (number, part), tensor in found.items():
+                if part == "A":
+                    a[number, :tensor.shape[0]] = tensor
+                else:
+                    b[number, :, :tensor.shape[1]] = tensor
+            has = [s if (n, "A") in found else 0.0 for n, s in enumerate(scalings)]
+            self._layers[layer] = (a, b, torch.tensor(has, dtype=torch.float32).to(device))
+
+    def holds(self, *layers):
+        """Whether any of these layers has an adapter here."""
+        return any(layer in self._layers for layer in layers)
+
+    def apply(self, x, index, pairs):
+        """y += scaling * (x @ A^T) @ B^T in place for every (layer, y) of `pairs` that has adapters, row m with adapter index[m] (int32; a negative
+        one adds nothing).  x fp16 [rows, in_features], y fp16 [rows, out_features]; up to four layers share x and a launch."""
+        specs = [self._layers[layer] + (y,) for layer, y in pairs if layer in self._layers]
+        by_rank = {}
+        for spec in specs:
+            by_rank.setdefault(spec[0].shape[1], []).append(spec)
+        for same in by_rank.values():                        # one launch holds layers of one rank
+            autograd_4bit.quant_hip.lora_rows(x, index, same)
