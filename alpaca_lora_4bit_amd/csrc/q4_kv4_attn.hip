@@ -326,9 +326,11 @@ __global__ __launch_bounds__(256, 3) void kv4_attn_rows_kernel(Kv4Attn a) {
 constexpr float kSlack = 5.0f;
 constexpr int kPromptRows = 128;
 
+constexpr int kHalfPiece = 36;                                             // keys: 32 pieces and room for four, so that a key's quarters are written to banks of their own
+
 template <int D>
 struct Kv4Staged {
-    uint4_t k[2 * D / 16 * 64], v[4 * D / 32 * 64];
+    uint4_t k[4 * D / 16 * kHalfPiece], v[4 * D / 32 * 64];
 };
 
 template <int D, int NG>
@@ -376,43 +378,60 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
             for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
         float m = -INFINITY, l = 0.f;
 
-        // This thread's part of a tile: a quarter of the words of key 16*wave + c, and word c of the four keys of block 4*wave + kk: all in run `wave`.
+        // This thread's part of a tile: quarter lane % 4 of the words of key 16*wave + lane / 4, and word c of the four keys of block 4*wave + kk: all in run
+        // `wave`, a contiguous kilobyte each.
         // Two tiles are on their way, and the page of the one behind them.
-        const int c = lane & 15, kk = lane >> 4;
+        const int c = lane & 15, kk = lane >> 4, kc = lane >> 2, kq = lane & 3;
         struct Raw {
             uint32_t k[S];
             uint4_t v;
             half_t ks[NG];
             half4_t vs[NG];
-            bool have;
+            int have;                                                      // -1 or 0
         } raw[2];
         int page = -1;                                                     // of the next tile to be requested
-        auto page_of = [&](int tile) {                                     // uniform
-            const int run = tile * 4 + wave;
-            return tile < t_end && run * 16 < kend ? table[a.page_magic ? (int)__umulhi((uint32_t)run, a.page_magic) : run] : -1;
-        };
-        auto request = [&](Raw& x, int tile) {
-            const int run = tile * 4 + wave;
-            const int idx = a.page_magic ? (int)__umulhi((uint32_t)run, a.page_magic) : run;
-            x.have = page >= 0 && page < a.c.pages;
-            const uint32_t head = (uint32_t)(x.have ? page : 0) * a.c.heads + h, off = x.have ? run - idx * p16 : 0;
+        int zero;                                                          // opaque: the page is loaded into a vector register and waited for where it is used
+        asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+        const int single = a.page_magic ? 0 : -1;                          // no branch in a tile's way: a taken one costs what fifty operations do
+        auto index_of = [&](int run) { return (int)__umulhi((uint32_t)run, a.page_magic) | (run & single); };
+        auto page_of = [&](int tile) { return table[index_of(min(tile * 4 + wave, (kend - 1) / 16)) + zero]; };   // of the tile's run, or of the last run there is
+        size_t words = 0, halves = 0;                                      // where the tile's run lies in a head's codes and scales
+        auto request_keys = [&](Raw& x, int tile) {
+            const int run = tile * 4 + wave, pg = __builtin_amdgcn_readfirstlane(page);
+            const int ok = -(int)((tile < t_end) & (run * 16 < kend) & ((uint32_t)pg < (uint32_t)a.c.pages));
+            x.have = ok;
+            const uint32_t head = (uint32_t)(pg & ok) * a.c.heads + h, off = (run - index_of(run) * p16) & ok;
             page = page_of(tile + 1);
-            const uint32_t* kp = a.c.kc + (size_t)(head * p16 + off) * (16 * W) + c * W + kk * S;
+            words = (size_t)(head * p16 + off) * (16 * W);
+            halves = ((size_t)head * NG * p16 + off) * 16;
+            const uint32_t* kp = a.c.kc + words + kc * W + kq * S;
             if constexpr (S == 4) *reinterpret_cast<uint4_t*>(x.k) = *reinterpret_cast<const uint4_t*>(kp);
             else *reinterpret_cast<uint2_t*>(x.k) = *reinterpret_cast<const uint2_t*>(kp);
-            x.v = *reinterpret_cast<const uint4_t*>(a.c.vc + (size_t)(head * p16 + off) * (16 * W) + (kk * W + c % W) * 4);
-            const size_t sc = ((size_t)head * NG * p16 + off) * 16;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                x.ks[g] = a.c.ks[sc + (size_t)g * a.c.page + c];
-                x.vs[g] = *reinterpret_cast<const half4_t*>(a.c.vs + sc + (size_t)g * a.c.page + 4 * kk);
-            }
+            for (int g = 0; g < NG; ++g) x.ks[g] = a.c.ks[halves + (size_t)g * a.c.page + kc];
+        };
+        auto request_values = [&](Raw& x) { x.v = *reinterpret_cast<const uint4_t*>(a.c.vc + words + (kk * W + c % W) * 4); };
+        auto request_scales = [&](Raw& x) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) x.vs[g] = *reinterpret_cast<const half4_t*>(a.c.vs + halves + (size_t)g * a.c.page + 4 * kk);
+        };
+        auto request = [&](Raw& x, int tile) {
+            request_keys(x, tile);
+            request_values(x);
+            request_scales(x);
         };
         // What no row of the workgroup sees is nothing, and a value's scale that is no number makes the rows none that see it.
         auto look = [&](Raw& x, int buf, int tile) {
             const int key = tile * 64 + 16 * wave;
-            if (lane == 0) there[buf][wave] = x.have || key >= kend;
-            const int ks_in = x.have ? kend - key - c : 0, vs_in = x.have ? kend - key - 4 * kk : 0;
+            there[buf][wave] = x.have | -(int)(key >= kend);
+            uint32_t odd = 0;                                              // the sign of a half: an exponent of all ones
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const uint2_t w = __builtin_bit_cast(uint2_t, x.vs[g]);
+                odd |= ((w.x & 0x7C007C00u) + 0x04000400u) | ((w.y & 0x7C007C00u) + 0x04000400u);
+            }
+            if (__builtin_expect((key + 16 <= kend) & (__ballot((odd & 0x80008000u) != 0) == 0) & (x.have != 0), 1)) return;
+            const int ks_in = x.have ? kend - key - kc : 0, vs_in = x.have ? kend - key - 4 * kk : 0;
             int strange = 0x7FFFFFFF;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
@@ -427,78 +446,71 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
             if (__any(strange != 0x7FFFFFFF)) atomicMin(&poison, strange);
         };
         const int kb_w = wave >> 1;                                        // the half of a tile that this wavefront's keys lie in
-        auto stage_keys = [&](const Raw& x, int buf) {
-            const int kr = 16 * (wave & 1) + c;
-#pragma unroll
-            for (int s = 0; s < S; ++s) {                                  // dimensions 32*s + 8*kk .. + 7
-                const half2_t f = {x.ks[s / SG], x.ks[s / SG]};
-                const uint4_t y = {as_u32(kv4_pair<0>(x.k[s]) * f), as_u32(kv4_pair<1>(x.k[s]) * f), as_u32(kv4_pair<2>(x.k[s]) * f),
-                                   as_u32(kv4_pair<3>(x.k[s]) * f)};
-                tiles_lds[buf].k[(kb_w * ST + 2 * s + (kk >> 1)) * 64 + 32 * (kk & 1) + kr] = y;
-            }
+        const int kr_w = 16 * (wave & 1) + kc;
+        auto stage_keys = [&](const Raw& x, int buf, int s) {              // dimensions 32*s + 8*kq .. + 7
+            const half2_t f = {x.ks[s / SG], x.ks[s / SG]};
+            const uint4_t y = {as_u32(kv4_pair<0>(x.k[s]) * f), as_u32(kv4_pair<1>(x.k[s]) * f), as_u32(kv4_pair<2>(x.k[s]) * f),
+                               as_u32(kv4_pair<3>(x.k[s]) * f)};
+            tiles_lds[buf].k[((kb_w * ST + 2 * s) * 2 + kq) * kHalfPiece + kr_w] = y;
         };
-        auto stage_values = [&](const Raw& x, int buf) {
-            // block 4*wave + kk of the tile: keys 4*kk .. of this half of its 32; piece p = wave & 1, h = kk & 1, half of it kk >> 1
+        uint32_t pr[2][2];                                                 // [pair of keys][even, odd nibbles]
+        auto pair_values = [&](const Raw& x) {
             uint32_t wd[4] = {x.v.x, x.v.y, x.v.z, x.v.w};
             if constexpr (D == 64) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) wd[e] >>= 16 * (c >> 3);
             }
-            uint32_t pr[2][2];                                             // [pair of keys][even, odd nibbles]
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 pr[q][0] = (wd[2 * q] & 0x0F0F0F0Fu) | ((wd[2 * q + 1] << 4) & 0xF0F0F0F0u);
                 pr[q][1] = ((wd[2 * q] >> 4) & 0x0F0F0F0Fu) | (wd[2 * q + 1] & 0xF0F0F0F0u);
             }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {                                 // dimension 16*i + c
-                uint2_t y;
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const uint32_t w = pr[q][i & 1];
-                    const half2_t f = {x.vs[i / HG][2 * q], x.vs[i / HG][2 * q + 1]};
-                    const half2_t d = i / 2 == 0 ? kv4_pair<0>(w) : i / 2 == 1 ? kv4_pair<1>(w) : i / 2 == 2 ? kv4_pair<2>(w) : kv4_pair<3>(w);
-                    y[q] = as_u32(d * f);
-                }
-                uint4_t* at = &tiles_lds[buf].v[((kb_w * 2 + (wave & 1)) * DB + i / 2) * 64 + 32 * (kk & 1) + 16 * (i & 1) + c];
-                reinterpret_cast<uint2_t*>(at)[kk >> 1] = y;
-            }
         };
-        // Tile t from half BUF, while t + 1 goes to the other one; behind the last tile that is written once more, for nobody.
+        // dimension 16*i + c of block 4*wave + kk of the tile: keys 4*kk .. of this half of its 32; piece p = wave & 1, h = kk & 1, half of it kk >> 1
+        auto stage_values = [&](const Raw& x, int buf, int i) {
+            uint2_t y;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const uint32_t w = pr[q][i & 1];
+                const half2_t f = {x.vs[i / HG][2 * q], x.vs[i / HG][2 * q + 1]};
+                const half2_t d = i / 2 == 0 ? kv4_pair<0>(w) : i / 2 == 1 ? kv4_pair<1>(w) : i / 2 == 2 ? kv4_pair<2>(w) : kv4_pair<3>(w);
+                y[q] = as_u32(d * f);
+            }
+            uint4_t* at = &tiles_lds[buf].v[((kb_w * 2 + (wave & 1)) * DB + i / 2) * 64 + 32 * (kk & 1) + 16 * (i & 1) + c];
+            reinterpret_cast<uint2_t*>(at)[kk >> 1] = y;
+        };
+        // Tile t from half BUF, while t + 1 goes to the other one; behind the last tile that is written once more, for nobody.  What goes between the
+        // products stands there: the compiler alone reads an operand, waits for it and multiplies.
         auto step = [&](auto half, int t) {
-            constexpr int BUF = decltype(half)::value;
+            constexpr int BUF = decltype(half)::value, N = 2 * ST, AHEAD = NG == 4 ? 3 : 4;   // N products of keys, and N of values
             const Kv4Staged<D>& x = tiles_lds[BUF];
             Raw& next = raw[BUF ^ 1];
-            const int th[4] = {there[BUF][0], there[BUF][1], there[BUF][2], there[BUF][3]};
+            half8_t op[AHEAD];
+            auto operand = [&](int i) {                                    // of product i: keys' (st, kb), then values' (kb, p, i)
+                op[i % AHEAD] = __builtin_bit_cast(half8_t, i < N ? x.k[((i & 1) * ST + (i >> 1)) * 2 * kHalfPiece + lane + h32 * (kHalfPiece - 32)] : x.v[(i - N) * 64 + lane]);
+            };
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) operand(i);
+            const int mine = there[BUF][lane & 3];
             look(next, BUF ^ 1, t + 1);
             float16_t s[2];
-            __builtin_amdgcn_sched_barrier(0);
-            stage_keys(next, BUF ^ 1);
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+            for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = 0.f;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
-#pragma unroll
-                for (int st = 0; st < ST; ++st)
-                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, x.k[(kb * ST + st) * 64 + lane]), qf[st], s[kb], 0, 0, 0);
+            for (int i = 0; i < N; ++i) {
+                s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[i % AHEAD], qf[i >> 1], s[i & 1], 0, 0, 0);
+                operand(i + AHEAD);
+                if (i % 4 == 3) stage_keys(next, BUF ^ 1, i / 4);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            // the conversion of the next keys goes between the products, operands three products ahead
-            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-#pragma unroll
-            for (int i = 0; i < 2 * ST; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-                __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            if (t * 64 + 64 > kmin || !(th[0] & th[1] & th[2] & th[3])) {  // register e of block kb: key 32*kb + 8*(e/4) + 4*h32 + e%4
+            const uint32_t gone = (uint32_t)__ballot(!mine) & 15u;         // runs that are not there
+            if (__builtin_expect((t * 64 + 64 > kmin) | (gone != 0), 0)) {                             // register e of block kb: key 32*kb + 8*(e/4) + 4*h32 + e%4
                 const int seen = limit - (t * 64 + 4 * h32);
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const int until = th[2 * kb + (e >> 3)] ? seen : 0;
+                        const int until = gone >> (2 * kb + (e >> 3)) & 1 ? 0 : seen;
                         s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) < until ? s[kb][e] : -INFINITY;
                     }
             }
@@ -506,7 +518,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
 #pragma unroll
             for (int e = 1; e < 32; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
             mx = max_of_halves(mx) * a.scale;
-            if (__any(mx > m + kSlack)) {
+            if (__builtin_expect(__any(mx > m + kSlack), 0)) {
                 const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
                 l *= f;
 #pragma unroll
@@ -515,49 +527,34 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
             }
             const float base = kBoost - (m == -INFINITY ? 0.f : m);
             uint4_t pw[4];
-            auto weights = [&](int kb) {
-                float part = 0.f;
+            auto weights = [&](int e) {                                    // e, e + 1 of the 32
+                float p[2];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], a.scale, base));
-                    part += s[kb][e];
+                for (int d = 0; d < 2; ++d) {
+                    p[d] = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][(e & 15) + d], a.scale, base));
+                    l += p[d];
                 }
-                l += part;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) pw[2 * kb + (e >> 2)][e & 3] = rounded_pair(s[kb][2 * e], s[kb][2 * e + 1]);
+                pw[e >> 3][(e & 7) >> 1] = rounded_pair(p[0], p[1]);
             };
-            auto values = [&](int kb) {
 #pragma unroll
-                for (int p = 0; p < 2; ++p)
-#pragma unroll
-                    for (int i = 0; i < DB; ++i)
-                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, x.v[((kb * 2 + p) * DB + i) * 64 + lane]),
-                                                                      __builtin_bit_cast(half8_t, pw[2 * kb + p]), o[i], 0, 0, 0);
-            };
-            weights(0);
+            for (int e = 0; e < 8; e += 2) weights(e);
             __builtin_amdgcn_sched_barrier(0);
-            values(0);
-            weights(1);
-            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
-            for (int i = 0; i < 2 * DB; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+            for (int i = 0; i < N; ++i) {
+                o[i % DB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[(N + i) % AHEAD], __builtin_bit_cast(half8_t, pw[i / DB]), o[i % DB], 0, 0, 0);
+                if (i + AHEAD < N) operand(N + i + AHEAD);
+                if (i < 3 * DB) {
+#pragma unroll
+                    for (int e = 0; e < 8 / DB; e += 2) weights(8 + i * (8 / DB) + e);
+                    asm volatile("" : "+v"(l));                            // the sum here, not behind all products
+                }
+                if (i == N / 2 - 1) pair_values(next);
+                if (i >= N / 2) stage_values(next, BUF ^ 1, i - N / 2);
+                if (i == 1) request_keys(next, t + 3);                     // their registers are free, and later those of the values
+                if (i == N / 2) request_values(next);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
-            values(1);
-            stage_values(next, BUF ^ 1);
-            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-#pragma unroll
-            for (int i = 0; i < 2 * DB; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
-                __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            request(next, t + 3);
+            request_scales(next);
             __syncthreads();
         };
 
@@ -567,16 +564,22 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
             request(raw[0], t0);
             request(raw[1], t0 + 1);
             look(raw[0], 0, t0);
-            stage_keys(raw[0], 0);
-            stage_values(raw[0], 0);
+#pragma unroll
+            for (int s = 0; s < S; ++s) stage_keys(raw[0], 0, s);
+            pair_values(raw[0]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) stage_values(raw[0], 0, i);
             request(raw[0], t0 + 2);
         }
+#pragma unroll
+        for (int s = 0; s < ST; ++s) asm volatile("" : "+v"(qf[s]));       // the queries have arrived: the loop does not wait for them
         __syncthreads();
-        for (int t = t0; t < t_end; t += 2) {
+        int t = t0;
+        for (; t + 1 < t_end; t += 2) {                                    // (a way out between the two would have every step wait for all requests)
             step(std::integral_constant<int, 0>{}, t);
-            if (t + 1 >= t_end) break;
             step(std::integral_constant<int, 1>{}, t + 1);
         }
+        if (t < t_end) step(std::integral_constant<int, 0>{}, t);
         if (limit > poison) l = NAN;
         {
             const uint32_t lb = __builtin_bit_cast(uint32_t, l);
