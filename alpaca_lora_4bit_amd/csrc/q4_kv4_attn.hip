@@ -346,7 +346,25 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
     id /= a.c.heads;
     const int split = id % a.nsplit;
     id /= a.nsplit;
-    const int b = id % a.p.B, block0 = a.blocks - 1 - id / a.p.B;          // the rows with the most keys first
+    // The rows with the most keys first.  Of up to 64 sequences the longest comes first with all its rows, so that its workgroups find compute units of their
+    // own and the short ones come beside them (parts of four prompts at 8191, 6995, 5062 and 1933 tokens: 238 us in turns, 195 sorted).
+    int b = id % a.p.B, block0 = a.blocks - 1 - id / a.p.B;
+    if (a.p.B > 1 && a.p.B <= 64) {
+        int mine = 0, length = -1, before = 0;                             // lane: a sequence, its blocks, and those of longer ones
+        if (lane < a.p.B) {
+            const int rows = (a.p.starts ? a.p.starts[lane + 1] - a.p.starts[lane] : a.p.T / a.p.B) * a.share;
+            mine = min((max(rows, 0) + kPromptRows - 1) / kPromptRows, a.blocks);
+            length = a.p.lengths[lane];
+        }
+        for (int k = 0; k < a.p.B; ++k) {
+            const int other = __builtin_amdgcn_readlane(length, k), blocks = __builtin_amdgcn_readlane(mine, k);
+            before += other > length || (other == length && k < lane) ? blocks : 0;
+        }
+        const uint64_t found = __ballot(lane < a.p.B && id >= before && id < before + mine);
+        if (!found) return;
+        b = __builtin_ctzll(found);
+        block0 = __builtin_amdgcn_readlane(before + mine, b) - 1 - id;
+    }
     const int first = a.p.starts ? a.p.starts[b] : b * (a.p.T / a.p.B);
     const int n = min((a.p.starts ? a.p.starts[b + 1] : (b + 1) * (a.p.T / a.p.B)) - first, a.p.T);
     const int len = a.p.lengths[b], cap = a.p.width * a.c.page, p16 = a.c.page / 16;
