@@ -666,12 +666,16 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4Attn a) {
     sum = (red[4] + red[5]) + (red[6] + red[7]);
     const int d = threadIdx.x % DV * 4, s0 = threadIdx.x / DV;
     float4_t v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = s0; s < a.nsplit; s += PER) {
-        const float w = wt[s];
-        if (w == 0.f) continue;
-        const float4_t x = *reinterpret_cast<const float4_t*>(a.part + (s * all + row) * D + d);
+    for (int s = s0; s < a.nsplit; s += 4 * PER) {
+        float4_t x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fmaf(w, x[e], v[e]);
+        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const float4_t*>(a.part + (min(s + k * PER, a.nsplit - 1) * all + row) * D + d);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float w = s + k * PER < a.nsplit ? wt[s + k * PER] : 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(w, w == 0.f ? 0.f : x[k][e], v[e]);
+        }
     }
     *reinterpret_cast<float4_t*>(&acc[s0][d]) = v;
     __syncthreads();
@@ -686,15 +690,16 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4Attn a) {
 // ---- plan ----------------------------------------------------------------------------------------
 struct Kv4AttnPlan { bool prompt; int blocks, nsplit; };
 
-// Above 64 rows a key head and sequence the prompt kernel, below it 16 rows a workgroup.  The keys are split until about four (prompts: two)
-// workgroups stand for every compute unit, a share of 256 keys (a tile per wavefront) at least.
+// Above 64 rows a key head and sequence the prompt kernel, below it 16 rows a workgroup.  The keys are split, a share of 256 keys (a tile per wavefront) at
+// least, until two prompts' workgroups or two of one sequence stand for every compute unit (131072 tokens of one: 31.9 us with 512 workgroups, 34.1 with 1024, 39.1
+// with 2048, for the shares are joined), eight of four sequences or more, whose lengths differ (32 of up to 16384: 101.7, 82.3 and 77.2 us).
 inline Kv4AttnPlan plan_kv4_attn(int B, int heads, int share, int max_tokens, int max_length) {
     Kv4AttnPlan p;
     const long rows = (long)max_tokens * share;
     p.prompt = rows > 64;
     const int per = p.prompt ? kPromptRows : 16;
     p.blocks = (int)((rows + per - 1) / per);
-    const long groups = (long)B * heads * p.blocks, wanted = p.prompt ? 512 : 1024;
+    const long groups = (long)B * heads * p.blocks, wanted = p.prompt ? 512 : std::min(512l * B, 2048l);
     const long most = std::max(1l, (max_length + 255l) / 256);
     p.nsplit = (int)std::max(1l, std::min({most, (wanted + groups - 1) / groups, 256l}));
     return p;
