@@ -39,12 +39,14 @@ struct Kv4Append {
     long k_t, k_h, v_t, v_h, q_t, q_h;
     const float* rope;                // [rope_rows][rot/2][2]; rot 0: no rotation
     int rope_rows, rot, interleaved, hq;
+    int turns;                        // heads a wavefront takes one after the other
 };
 
 struct Kv4Read {
     Kv4Cache c;
     Kv4Batch p;
     half_t *k, *v;                    // [T, heads, D]
+    int turns;
 };
 
 struct Kv4Attn {
