@@ -4,7 +4,7 @@
 //
 // One pass over the keys with the running maximum m and sum l of the softmax in fp32.  Codes go to the matrix instructions as the exact
 // fp16 values that they stand for; the keys' scales multiply the fp32 scores, the values' scales the probabilities, whose rounding to
-// fp16 is the only one before the output's.
+// fp16 is the only one before the output's (prompts round more, see there).
 #include "q4_kv4.hpp"
 #include <algorithm>
 #include <type_traits>
@@ -317,14 +317,25 @@ __global__ __launch_bounds__(256, 3) void kv4_attn_rows_kernel(Kv4Attn a) {
 }
 
 // ---- prompts: 128 rows a workgroup -----------------------------------------------------------------
-// Four wavefronts of 32 rows on the same tiles of 64 keys.  The workgroup turns a tile's codes into fp16 values (one rounding each, of code * scale) in LDS, in
-// the order in which v_mfma_f32_32x32x16_f16 takes them: pieces of 16 bytes, lane after lane, so that neither side meets a bank conflict.  Two tiles: the next one
-// is written, and the one behind it requested, while one is multiplied; one barrier a tile.  As above S^T = K Q^T and O^T = V^T P^T, lane (r, h) holding row r:
+// Four wavefronts of 32 rows on the same tiles of 64 keys.  The workgroup turns a tile's codes into fp16 values (values: one rounding each, of code * scale) in LDS,
+// in the order in which v_mfma_f32_32x32x16_f16 takes them: pieces of 16 bytes, lane after lane, so that neither side meets a bank conflict.  Two tiles: the next one
+// is written, and the two behind it requested, while one is multiplied; one barrier a tile.  As above S^T = K Q^T and O^T = V^T P^T, lane (r, h) holding row r:
 //   keys' piece (kb, st, lane): key 32*kb + r, dimensions 16*st + 8*h .. + 7
 //   values' piece (kb, p, db, lane): dimension 32*db + r of keys 32*kb + 16*p + 4*h + (0..3) and + 8, the keys of the scores in that lane's registers 8*p .. + 7
 // The maximum that weights refer to is raised only when a score lies 2^kSlack above it: weights then stay below 2^15.
+//
+// Rows that see up to kFewKeys keys get the keys' codes as they are, and each group's fp32 sums times its keys' scales; for rows that see more, code * scale is
+// rounded once like the values.  Root mean square error of a whole output against float64, relative: 2.6e-4 so, 3.1e-4 with all rounded for the prompt of 2048 tokens, 2.6e-4 and 3.4e-4
+// for one of 128 (2.1e-4 are the output's own rounding), but 2.4e-4 rounded where 4096 keys average it; exact keys cost 5, 15 and 40 per cent at 1, 2 and 4 groups.
+//
+// What bounds it: a wavefront starts an operation in about eight cycles, and two of them share a SIMD, whose vector operations (230 a tile and wavefront) and matrix
+// operations (32 of 32 cycles) take 1900 of the 3250 to 4400 cycles that a tile of both lasts at 2.1 GHz.  The whole prompt of 2048 tokens, 32 heads of 128: 64 us, of which the
+// last block's 32 tiles are 55; parts of four prompts (509, 434, 360, 286 tokens at 8191, 5062, 1933, 6995; 8 key heads of 4): 195 us, 128 tiles one after the other.
+// Eight wavefronts on 256 rows, half turning keys, half values: 69 and 216 us, for all are at the same step; splitting the keys of whole prompts costs the join more
+// than the balance gives (parts: 271 us in two shares).
 constexpr float kSlack = 5.0f;
 constexpr int kPromptRows = 128;
+constexpr int kFewKeys = 1024;
 
 constexpr int kHalfPiece = 36;                                             // keys: 32 pieces and room for four, so that a key's quarters are written to banks of their own
 
@@ -337,6 +348,7 @@ template <int D, int NG>
 __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
     constexpr int S = D / 32, ST = D / 16, DB = D / 32, W = D / 8, SG = S / NG, H = D / 16, HG = H / NG, NV = D / 16;   // NV: nibbles of a word a thread takes
     __shared__ __attribute__((aligned(16))) Kv4Staged<D> tiles_lds[2];
+    __shared__ __attribute__((aligned(16))) float key_scales[2][NG][64];
     __shared__ int poison;                                                 // first key seen whose values are no numbers
     __shared__ int there[2][4];                                            // whether the tile's runs of 16 keys lie on pages of the cache
     const int lane = threadIdx.x & 63, r = lane & 31, h32 = lane >> 5;
@@ -411,10 +423,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
         int zero;                                                          // opaque: the page is loaded into a vector register and waited for where it is used
         asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
         const int single = a.page_magic ? 0 : -1;                          // no branch in a tile's way: a taken one costs what fifty operations do
-        auto index_of = [&](int run) { return (int)__umulhi((uint32_t)run, a.page_magic) | (run & single); };
-        auto page_of = [&](int tile) { return table[index_of(min(tile * 4 + wave, (kend - 1) / 16)) + zero]; };   // of the tile's run, or of the last run there is
+        auto index_of = [&](int run) __attribute__((always_inline)) { return (int)__umulhi((uint32_t)run, a.page_magic) | (run & single); };
+        auto page_of = [&](int tile) __attribute__((always_inline)) { return table[index_of(min(tile * 4 + wave, (kend - 1) / 16)) + zero]; };   // of the tile's run, or of the last run there is
         size_t words = 0, halves = 0;                                      // where the tile's run lies in a head's codes and scales
-        auto request_keys = [&](Raw& x, int tile) {
+        auto request_keys = [&](Raw& x, int tile) __attribute__((always_inline)) {
             const int run = tile * 4 + wave, pg = __builtin_amdgcn_readfirstlane(page);
             const int ok = -(int)((tile < t_end) & (run * 16 < kend) & ((uint32_t)pg < (uint32_t)a.c.pages));
             x.have = ok;
@@ -428,18 +440,18 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
 #pragma unroll
             for (int g = 0; g < NG; ++g) x.ks[g] = a.c.ks[halves + (size_t)g * a.c.page + kc];
         };
-        auto request_values = [&](Raw& x) { x.v = *reinterpret_cast<const uint4_t*>(a.c.vc + words + (kk * W + c % W) * 4); };
-        auto request_scales = [&](Raw& x) {
+        auto request_values = [&](Raw& x) __attribute__((always_inline)) { x.v = *reinterpret_cast<const uint4_t*>(a.c.vc + words + (kk * W + c % W) * 4); };
+        auto request_scales = [&](Raw& x) __attribute__((always_inline)) {
 #pragma unroll
             for (int g = 0; g < NG; ++g) x.vs[g] = *reinterpret_cast<const half4_t*>(a.c.vs + halves + (size_t)g * a.c.page + 4 * kk);
         };
-        auto request = [&](Raw& x, int tile) {
+        auto request = [&](Raw& x, int tile) __attribute__((always_inline)) {
             request_keys(x, tile);
             request_values(x);
             request_scales(x);
         };
         // What no row of the workgroup sees is nothing, and a value's scale that is no number makes the rows none that see it.
-        auto look = [&](Raw& x, int buf, int tile) {
+        auto look = [&](Raw& x, int buf, int tile) __attribute__((always_inline)) {
             const int key = tile * 64 + 16 * wave;
             there[buf][wave] = x.have | -(int)(key >= kend);
             uint32_t odd = 0;                                              // the sign of a half: an exponent of all ones
@@ -465,14 +477,19 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
         };
         const int kb_w = wave >> 1;                                        // the half of a tile that this wavefront's keys lie in
         const int kr_w = 16 * (wave & 1) + kc;
-        auto stage_keys = [&](const Raw& x, int buf, int s) {              // dimensions 32*s + 8*kq .. + 7
-            const half2_t f = {x.ks[s / SG], x.ks[s / SG]};
-            const uint4_t y = {as_u32(kv4_pair<0>(x.k[s]) * f), as_u32(kv4_pair<1>(x.k[s]) * f), as_u32(kv4_pair<2>(x.k[s]) * f),
-                               as_u32(kv4_pair<3>(x.k[s]) * f)};
+        auto stage_keys = [&](auto exact, const Raw& x, int buf, int s) __attribute__((always_inline)) {  // dimensions 32*s + 8*kq .. + 7
+            uint4_t y;
+            if constexpr (decltype(exact)::value) {
+                y = __builtin_bit_cast(uint4_t, kv4_word(x.k[s]));
+                if (s % SG == 0) key_scales[buf][s / SG][16 * wave + kc] = (float)x.ks[s / SG];
+            } else {
+                const half2_t f = {x.ks[s / SG], x.ks[s / SG]};
+                y = uint4_t{as_u32(kv4_pair<0>(x.k[s]) * f), as_u32(kv4_pair<1>(x.k[s]) * f), as_u32(kv4_pair<2>(x.k[s]) * f), as_u32(kv4_pair<3>(x.k[s]) * f)};
+            }
             tiles_lds[buf].k[((kb_w * ST + 2 * s) * 2 + kq) * kHalfPiece + kr_w] = y;
         };
         uint32_t pr[2][2];                                                 // [pair of keys][even, odd nibbles]
-        auto pair_values = [&](const Raw& x) {
+        auto pair_values = [&](const Raw& x) __attribute__((always_inline)) {
             uint32_t wd[4] = {x.v.x, x.v.y, x.v.z, x.v.w};
             if constexpr (D == 64) {
 #pragma unroll
@@ -485,7 +502,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
             }
         };
         // dimension 16*i + c of block 4*wave + kk of the tile: keys 4*kk .. of this half of its 32; piece p = wave & 1, h = kk & 1, half of it kk >> 1
-        auto stage_values = [&](const Raw& x, int buf, int i) {
+        auto stage_values = [&](const Raw& x, int buf, int i) __attribute__((always_inline)) {
             uint2_t y;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
@@ -499,30 +516,46 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
         };
         // Tile t from half BUF, while t + 1 goes to the other one; behind the last tile that is written once more, for nobody.  What goes between the
         // products stands there: the compiler alone reads an operand, waits for it and multiplies.
-        auto step = [&](auto half, int t) {
-            constexpr int BUF = decltype(half)::value, N = 2 * ST, AHEAD = NG == 4 ? 3 : 4;   // N products of keys, and N of values
+        auto step = [&](auto exact, auto half, int t) __attribute__((always_inline)) {
+            constexpr bool EXACT = decltype(exact)::value;
+            constexpr int BUF = decltype(half)::value, N = 2 * ST, AHEAD = 3;   // N products of keys, and N of values
             const Kv4Staged<D>& x = tiles_lds[BUF];
             Raw& next = raw[BUF ^ 1];
             half8_t op[AHEAD];
-            auto operand = [&](int i) {                                    // of product i: keys' (st, kb), then values' (kb, p, i)
+            auto operand = [&](int i) __attribute__((always_inline)) {                                    // of product i: keys' (st, kb), then values' (kb, p, i)
                 op[i % AHEAD] = __builtin_bit_cast(half8_t, i < N ? x.k[((i & 1) * ST + (i >> 1)) * 2 * kHalfPiece + lane + h32 * (kHalfPiece - 32)] : x.v[(i - N) * 64 + lane]);
             };
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) operand(i);
             const int mine = there[BUF][lane & 3];
             look(next, BUF ^ 1, t + 1);
-            float16_t s[2];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = 0.f;
+            float16_t s[2], sum[2];
+            constexpr int RUN = EXACT ? N / NG : N;                        // products of a group's dimensions, then its scales
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[i % AHEAD], qf[i >> 1], s[i & 1], 0, 0, 0);
+                float16_t& y = EXACT ? sum[i & 1] : s[i & 1];
+                if (i % RUN < 2) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) y[e] = 0.f;
+                }
+                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[i % AHEAD], qf[i >> 1], y, 0, 0, 0);
                 operand(i + AHEAD);
-                if (i % 4 == 3) stage_keys(next, BUF ^ 1, i / 4);
+                if (i % 4 == 3) stage_keys(exact, next, BUF ^ 1, i / 4);
                 __builtin_amdgcn_sched_barrier(0);
+                if (EXACT && i % RUN == RUN - 1) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4_t f = *reinterpret_cast<const float4_t*>(&key_scales[BUF][i / RUN][32 * (e >> 4) + 2 * (e & 15) + 4 * h32]);
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            const float z = sum[e >> 4][(e & 15) + d];
+                            s[e >> 4][(e & 15) + d] = i < RUN ? z * f[d] : fmaf(z, f[d], s[e >> 4][(e & 15) + d]);
+                        }
+                    }
+                }
             }
             const uint32_t gone = (uint32_t)__ballot(!mine) & 15u;         // runs that are not there
-            if (__builtin_expect((t * 64 + 64 > kmin) | (gone != 0), 0)) {                             // register e of block kb: key 32*kb + 8*(e/4) + 4*h32 + e%4
+            if (__builtin_expect((t * 64 + 64 > kmin) | (gone != 0), 0)) {  // register e of block kb: key 32*kb + 8*(e/4) + 4*h32 + e%4
                 const int seen = limit - (t * 64 + 4 * h32);
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
@@ -545,7 +578,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
             }
             const float base = kBoost - (m == -INFINITY ? 0.f : m);
             uint4_t pw[4];
-            auto weights = [&](int e) {                                    // e, e + 1 of the 32
+            auto weights = [&](int e) __attribute__((always_inline)) {                                    // e, e + 1 of the 32
                 float p[2];
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
@@ -577,27 +610,31 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
         };
 
         __syncthreads();
-        if (t0 < t_end) {
-            page = page_of(t0);
-            request(raw[0], t0);
-            request(raw[1], t0 + 1);
-            look(raw[0], 0, t0);
+        auto all = [&](auto exact) __attribute__((always_inline)) {
+            if (t0 < t_end) {
+                page = page_of(t0);
+                request(raw[0], t0);
+                request(raw[1], t0 + 1);
+                look(raw[0], 0, t0);
 #pragma unroll
-            for (int s = 0; s < S; ++s) stage_keys(raw[0], 0, s);
-            pair_values(raw[0]);
+                for (int s = 0; s < S; ++s) stage_keys(exact, raw[0], 0, s);
+                pair_values(raw[0]);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) stage_values(raw[0], 0, i);
-            request(raw[0], t0 + 2);
-        }
+                for (int i = 0; i < NV; ++i) stage_values(raw[0], 0, i);
+                request(raw[0], t0 + 2);
+            }
 #pragma unroll
-        for (int s = 0; s < ST; ++s) asm volatile("" : "+v"(qf[s]));       // the queries have arrived: the loop does not wait for them
-        __syncthreads();
-        int t = t0;
-        for (; t + 1 < t_end; t += 2) {                                    // (a way out between the two would have every step wait for all requests)
-            step(std::integral_constant<int, 0>{}, t);
-            step(std::integral_constant<int, 1>{}, t + 1);
-        }
-        if (t < t_end) step(std::integral_constant<int, 0>{}, t);
+            for (int s = 0; s < ST; ++s) asm volatile("" : "+v"(qf[s]));   // the queries have arrived: the loop does not wait for them
+            __syncthreads();
+            int t = t0;
+            for (; t + 1 < t_end; t += 2) {                                // (a way out between the two would have every step wait for all requests)
+                step(exact, std::integral_constant<int, 0>{}, t);
+                step(exact, std::integral_constant<int, 1>{}, t + 1);
+            }
+            if (t < t_end) step(exact, std::integral_constant<int, 0>{}, t);
+        };
+        if (kend <= kFewKeys) all(std::true_type{});
+        else all(std::false_type{});
         if (limit > poison) l = NAN;
         {
             const uint32_t lb = __builtin_bit_cast(uint32_t, l);
