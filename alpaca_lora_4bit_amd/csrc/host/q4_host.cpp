@@ -736,7 +736,7 @@ Kv4 check_kv4(const Kv4Tensors& c, const at::Tensor& table, const at::Tensor& le
     if (T > 0) {
         TORCH_CHECK_VALUE(B >= 1 && width >= 1 && width * page <= (1 << 26), "page_table must cover 1 to 2^26 tokens of at least one sequence");
         TORCH_CHECK_VALUE(sp || T % B == 0, "without starts every sequence has the same number of rows; got ", T, " rows of ", B, " sequences");
-        TORCH_CHECK_VALUE(T < (1ll << 31), "too many rows");
+        TORCH_CHECK_VALUE(T <= (1 << 24), "a call takes up to 2^24 rows, got ", T);
     }
     return Kv4{{kc.data_ptr<int>(), vc.data_ptr<int>(), ks.data_ptr(), vs.data_ptr(), (int)P, (int)page, (int)H, (int)D, (int)(D / NG)},
                {table.data_ptr<int>(), (int)width, lengths.data_ptr<int>(), sp, (int)B, (int)T}, dev};
@@ -753,11 +753,25 @@ at::Tensor check_heads(const at::Tensor& t, int64_t T, int64_t D, const c10::Dev
     return t;
 }
 
+// Whether the memory that two tensors span has bytes in common (strides are not negative).
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    auto last = [](const at::Tensor& t) {
+        int64_t n = 1;
+        for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+        return reinterpret_cast<uintptr_t>(t.data_ptr()) + n * t.element_size();
+    };
+    return reinterpret_cast<uintptr_t>(a.data_ptr()) < last(b) && reinterpret_cast<uintptr_t>(b.data_ptr()) < last(a);
+}
+
+// The result's tensor: a new one, or the caller's, which may be `like` itself but not another piece of its memory.
 at::Tensor rows_out(const c10::optional<at::Tensor>& out, int64_t T, int64_t H, int64_t D, const at::Tensor& like, const char* what) {
     if (!out.has_value()) return at::empty({T, H, D}, like.options());
     TORCH_CHECK_VALUE(out->scalar_type() == at::kHalf && out->dim() == 3 && out->size(0) == T && out->size(1) == H && out->size(2) == D &&
                       out->is_contiguous() && out->device() == like.device() && reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0, what,
                       " must be a contiguous, 16-byte aligned float16 [", T, ", ", H, ", ", D, "] tensor on the cache's device");
+    check_no_grad(*out, what);
+    TORCH_CHECK_VALUE((out->data_ptr() == like.data_ptr() && like.is_contiguous()) || !overlap(*out, like), what, " overlaps the queries");
     return *out;
 }
 
@@ -772,6 +786,7 @@ c10::optional<at::Tensor> kv4_append(const at::Tensor& k, const at::Tensor& v, c
     at::Tensor q3, o;
     if (q.has_value()) {
         q3 = check_heads(*q, T, c.cache.D, c.device, false, "q");
+        TORCH_CHECK_VALUE(!q_out.has_value() || (!overlap(*q_out, k) && !overlap(*q_out, v)), "q_out overlaps k or v");
         o = rows_out(q_out, T, q->size(1), c.cache.D, *q, "q_out");
     } else {
         TORCH_CHECK_VALUE(!q_out.has_value(), "q_out needs q");
@@ -862,6 +877,11 @@ void lora_rows(const at::Tensor& x, const at::Tensor& index, const std::vector<R
                           "scaling must be a contiguous float32 [n] tensor on x's device");
         TORCH_CHECK_VALUE(y.scalar_type() == at::kHalf && y.dim() == 2 && y.size(0) == M && y.size(1) == b.size(1) && y.is_contiguous() &&
                           y.device() == x.device(), "y must be a contiguous float16 [M, N] tensor on x's device");
+        check_no_grad(s, "scaling");
+        TORCH_CHECK_VALUE(!overlap(y, x) && !overlap(y, a) && !overlap(y, b), "y overlaps another tensor of the call");
+        for (size_t j = 0; j < i; ++j)
+            TORCH_CHECK_VALUE(!overlap(y, std::get<3>(specs[j])) && !overlap(y, std::get<0>(specs[j])) && !overlap(y, std::get<1>(specs[j])) &&
+                              !overlap(a, std::get<3>(specs[j])) && !overlap(b, std::get<3>(specs[j])), "y overlaps another tensor of the call");
         for (const at::Tensor* t : {&a, &b, &y}) {
             check_no_grad(*t, "a tensor of lora_rows");
             TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "the tensors of lora_rows must be 16-byte aligned");
@@ -870,7 +890,7 @@ void lora_rows(const at::Tensor& x, const at::Tensor& index, const std::vector<R
         probs[i] = {a.data_ptr(), b.data_ptr(), s.data_ptr<float>(), y.data_ptr(), (int)y.size(1)};
     }
     TORCH_CHECK_VALUE(R >= 8 && R <= 64 && R % 8 == 0, "the rank must be a multiple of 8 in [8, 64], got ", R);
-    TORCH_CHECK_VALUE(K >= 32 && K % 32 == 0 && K <= (1 << 20) && M < (1 << 30), "K must be a multiple of 32");
+    TORCH_CHECK_VALUE(K >= 32 && K % 32 == 0 && K <= (1 << 20) && M <= (1 << 24), "K must be a multiple of 32 up to 2^20, and x have up to 2^24 rows");
     TORCH_CHECK_VALUE(n < (1ll << 31) && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, "x must be 16-byte aligned");
     if (M == 0 || n == 0) return;
     Launch L(x.device());

@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Read a) {
     const int first = blockIdx.y * 4 * a.turns + (threadIdx.x >> 6);
     if (first >= 2 * heads) return;
     const Kv4Place w = kv4_place<L>(a.c, a.p, t);
-    if (!w.mine) return;
+    if (t >= a.p.T) return;                                                // a row of no sequence has no place
     for (int i = 0; i < a.turns; ++i) {
         int h = first + 4 * i;
         if (h >= 2 * heads) return;

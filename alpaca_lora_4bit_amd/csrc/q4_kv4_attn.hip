@@ -730,7 +730,7 @@ struct Kv4AttnPlan { bool prompt; int blocks, nsplit; };
 // Above 64 rows a key head and sequence the prompt kernel, below it 16 rows a workgroup.  The keys are split, a share of 256 keys (a tile per wavefront) at
 // least, until two prompts' workgroups or two of one sequence stand for every compute unit (131072 tokens of one: 31.9 us with 512 workgroups, 34.1 with 1024, 39.1
 // with 2048, for the shares are joined), eight of four sequences or more, whose lengths differ (32 of up to 16384: 101.7, 82.3 and 77.2 us).
-inline Kv4AttnPlan plan_kv4_attn(int B, int heads, int share, int max_tokens, int max_length) {
+inline Kv4AttnPlan plan_kv4_attn(int B, int heads, int D, int share, int T, int max_tokens, int max_length) {
     Kv4AttnPlan p;
     const long rows = (long)max_tokens * share;
     p.prompt = rows > 64;
@@ -738,14 +738,16 @@ inline Kv4AttnPlan plan_kv4_attn(int B, int heads, int share, int max_tokens, in
     p.blocks = (int)((rows + per - 1) / per);
     const long groups = (long)B * heads * p.blocks, wanted = p.prompt ? 512 : std::min(512l * B, 2048l);
     const long most = std::max(1l, (max_length + 255l) / 256);
-    p.nsplit = (int)std::max(1l, std::min({most, (wanted + groups - 1) / groups, 256l}));
+    // bounds that are right ask for 200 MB at most; others must not ask for all memory, nor for more rows than the join can be launched for
+    const long room = (1l << 30) / ((long)T * heads * share * (D + 2) * (long)sizeof(float));
+    p.nsplit = (int)std::max(1l, std::min({most, (wanted + groups - 1) / groups, 256l, room}));
     return p;
 }
 
 }  // namespace q4
 
 size_t q4_kv4_attn_workspace(int B, int heads, int D, int share, int T, int max_tokens, int max_length) {
-    const q4::Kv4AttnPlan p = q4::plan_kv4_attn(B, heads, share, max_tokens, max_length);
+    const q4::Kv4AttnPlan p = q4::plan_kv4_attn(B, heads, D, share, T, max_tokens, max_length);
     return p.nsplit == 1 ? 0 : (size_t)p.nsplit * T * heads * share * (D + 2) * sizeof(float);
 }
 
@@ -759,7 +761,7 @@ static void launch_attn(const q4::Kv4Attn& a, bool prompt, hipStream_t stream) {
 }
 
 int q4_launch_kv4_attn(q4::Kv4Attn& a, int D, int group, int max_tokens, int max_length, hipStream_t stream) {
-    const q4::Kv4AttnPlan p = q4::plan_kv4_attn(a.p.B, a.c.heads, a.share, max_tokens, max_length);
+    const q4::Kv4AttnPlan p = q4::plan_kv4_attn(a.p.B, a.c.heads, D, a.share, a.p.T, max_tokens, max_length);
     a.blocks = p.blocks;
     a.nsplit = p.nsplit;
     const uint32_t p16 = a.c.page / 16;

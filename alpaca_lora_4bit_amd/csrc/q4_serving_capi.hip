@@ -16,7 +16,7 @@ int check_cache(const q4_kv4_cache_t* c, const q4_kv4_batch_t* b) {
     // places are counted in units of 16 tokens of one head and group, in 31 bits
     if ((double)c->pages * c->heads * (c->page / 16) * (c->D / c->group) >= 2147483648.0) return Q4_ERR_BAD_SHAPE;
     if (b->width < 1 || (long long)b->width * c->page > (1ll << 26) || b->B < 1 || b->T < 1) return Q4_ERR_BAD_SHAPE;
-    if (!b->starts && b->T % b->B != 0) return Q4_ERR_BAD_SHAPE;
+    if (b->T > (1 << 24) || (!b->starts && b->T % b->B != 0)) return Q4_ERR_BAD_SHAPE;
     if (misaligned(c->k_codes) || misaligned(c->v_codes) || misaligned(c->k_scales) || misaligned(c->v_scales)) return Q4_ERR_MISALIGNED;
     return Q4_OK;
 }
@@ -90,7 +90,7 @@ extern "C" int q4_kv4_attention_f16(const q4_kv4_cache_t* cache, const q4_kv4_ba
 }
 
 static bool lora_rows_shape(int count, int M, int K, int R) {
-    return count >= 1 && count <= 4 && M >= 1 && K >= 32 && K % 32 == 0 && R >= 8 && R <= 64 && R % 8 == 0 && K <= (1 << 20) && M < (1 << 30);
+    return count >= 1 && count <= 4 && M >= 1 && K >= 32 && K % 32 == 0 && R >= 8 && R <= 64 && R % 8 == 0 && K <= (1 << 20) && M <= (1 << 24);
 }
 
 extern "C" size_t q4_lora_rows_workspace_bytes(int count, int M, int K, int R) {

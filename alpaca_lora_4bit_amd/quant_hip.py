@@ -1045,18 +1045,20 @@ def kv4_append(k, v, cache, page_table, lengths, q=None, rope=None, interleaved=
     """Stores k, v fp16 [rows, heads, D] (dimensions side by side, other strides free) as 4-bit values at the places of the batch's rows;
     `lengths` counts these tokens already.  rope fp32 [positions, rotated/2, 2] (cosine, sine): k, and q fp16 [rows, q_heads, D], are turned on
     the way, pairs (i, i + rotated/2), `interleaved` (2i, 2i + 1).  Returns the turned q (into `q_out` if given) or None.  A row whose position
-    or page does not exist is not stored and its q comes out as zero; rows of no sequence are not written."""
+    or page does not exist is not stored and its q comes out as zero; rows of no sequence are not written (a new result's are undefined).
+    `q_out` may be a contiguous q itself."""
     return _serving().kv4_append(k, v, cache, page_table, lengths, q, rope, bool(interleaved), starts, q_out)
 
 
 def kv4_read(cache, page_table, lengths, rows, starts=None):
-    """(k, v) fp16 [rows, heads, D]: what the cache holds at the places of the batch's rows; zero where a row has none."""
+    """(k, v) fp16 [rows, heads, D]: what the cache holds at the places of the batch's rows; zero where a row has none or belongs to no sequence."""
     return _serving().kv4_read(cache, page_table, lengths, int(rows), starts)
 
 
 def kv4_attention(q, cache, page_table, lengths, scale=None, starts=None, max_tokens=None, max_length=None, out=None):
     """fp16 [rows, q_heads, D]: attention of every row over its sequence's keys at or before its own position, softmax(scale * q . k) v
-    (scale None: 1/sqrt(D)).  A row that sees no key comes out as zero; rows of no sequence are not written.  `max_tokens`, the rows of the longest
+    (scale None: 1/sqrt(D)), into `out` if given, which may be a contiguous q itself.  A row that sees no key comes out as zero; rows of no sequence are
+    not written (a new result's are undefined).  `max_tokens`, the rows of the longest
     run of new tokens, and `max_length`, the tokens of the longest sequence, size the launch (None: what the shapes allow); the result does not
     depend on them being right."""
     if scale is None:
@@ -1069,7 +1071,8 @@ def kv4_attention(q, cache, page_table, lengths, scale=None, starts=None, max_to
 def lora_rows(x, index, specs, rows_per_index=1):
     """y += scaling[a] * (x @ A[a]^T) @ B[a]^T in place with a = index[m // rows_per_index] (int32 [ceil(M / rows_per_index)]) for every row m of
     x fp16 [M, K] and every (A fp16 [n, R, K], B fp16 [n, N, R], scaling fp32 [n], y fp16 [M, N]) of up to four layers that share x: the adapter of
-    each request beside a product that all of them share.  R is a multiple of 8 up to 64; rows whose index is not in 0 .. n - 1 keep their y."""
+    each request beside a product that all of them share.  R is a multiple of 8 up to 64; rows whose index is not in 0 .. n - 1 keep their y.  No y may
+    overlap another tensor of the call."""
     _serving().lora_rows(x, index, specs, int(rows_per_index))
 
 

@@ -383,7 +383,7 @@ typedef struct {
  * which counts lengths[b] tokens, these included, on the pages table[b][0 .. width-1] (width * page <= 2^26).  All three are device memory and are
  * read when the kernels run.  Whatever they hold, nothing outside the cache is touched: a row whose position is negative or behind the table, or whose
  * page is not one of 0 .. pages - 1, has no place; rows outside starts[0] .. starts[B] - 1 belong to no sequence.  Sequences share pages only if none of
- * the sharers appends to them. */
+ * the sharers appends to them.  T <= 2^24. */
 typedef struct {
     const int32_t *table;
     int width;
@@ -394,17 +394,17 @@ typedef struct {
 /* k, v fp16 (token and head strides in elements, dimensions side by side) go to the places of their rows; q (NULL: none) of q_heads heads comes out as
  * q_out fp16 [T, q_heads, D].  The first `rot` dimensions (a multiple of 16, 0: none) of k and q are turned by pairs (x_i, x_{i+rot/2}), `interleaved`
  * (x_{2i}, x_{2i+1}), with rope fp32 [rope_rows, rot/2, 2] = cosine and sine at the token's position; a position behind the table counts as no place.  A row
- * without a place is not stored and its q_out is zero; a row of no sequence leaves everything as it was. */
+ * without a place is not stored and its q_out is zero; a row of no sequence leaves everything as it was.  q_out may be q if that is contiguous. */
 Q4_API int q4_kv4_append_f16(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, const void *k, long long k_t, long long k_h,
                       const void *v, long long v_t, long long v_h, const void *q, long long q_t, long long q_h, void *q_out, int q_heads,
                       const float *rope, int rope_rows, int rot, int interleaved, void *stream);
 
-/* k, v fp16 [T, heads, D] = what the cache holds at the places of the batch's rows (zero without a place). */
+/* k, v fp16 [T, heads, D] = what the cache holds at the places of the batch's rows (zero without a place, rows of no sequence among them). */
 Q4_API int q4_kv4_read_f16(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, void *k, void *v, void *stream);
 
 /* out fp16 [T, q_heads, D]: attention of each row over its sequence's keys at or before its own position, softmax(scale * q . k) v with
  * q fp16 (strides as above, multiples of 8), q head h on key head h / (q_heads / heads).  A row that sees no key comes out as zero; keys without a
- * place are not seen.  scale > 0.  `max_tokens` (rows of the longest sequence) and `max_length` (its tokens) size the launch; the result does not depend on
+ * place are not seen.  scale > 0.  out may be q if that is contiguous.  `max_tokens` (rows of the longest sequence) and `max_length` (its tokens) size the launch; the result does not depend on
  * their being right.  `workspace`: the bytes that the query gives for the same arguments (0: may be NULL), 256-byte aligned, contents irrelevant. */
 Q4_API size_t q4_kv4_attention_workspace_bytes(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, int q_heads, int max_tokens, int max_length);
 Q4_API int q4_kv4_attention_f16(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, const void *q, long long q_t, long long q_h, int q_heads,
@@ -413,7 +413,7 @@ Q4_API int q4_kv4_attention_f16(const q4_kv4_cache_t *cache, const q4_kv4_batch_
 /* y_i fp16 [M, N_i] += scaling_i[a] * (x fp16 [M, K] @ A_i[a]^T) @ B_i[a]^T in place, a = index[m / per] (int32, device memory), for the
  * `count` (1..4) layers that share x and the index: the adapters of the requests of a batch beside the products that they share (models.py:58-66 adds one
  * adapter to all rows).  A_i fp16 [n, R, K], B_i fp16 [n, N_i, R], scaling_i fp32 [n]; R a multiple of 8 up to 64 (smaller adapters are filled up
- * with zeros), K % 32 == 0, N_i % 64 == 0.  Rows whose index lies outside 0 .. n - 1 are left as they are.  The y_i must not overlap.
+ * with zeros), K % 32 == 0, N_i % 64 == 0, M <= 2^24.  Rows whose index lies outside 0 .. n - 1 are left as they are.  The y_i must not overlap.
  * `workspace`: q4_lora_rows_workspace_bytes bytes, 256-byte aligned, contents irrelevant. */
 typedef struct { const void *a, *b; const float *scaling; void *y; int N; } q4_lora_rows_t;
 Q4_API size_t q4_lora_rows_workspace_bytes(int count, int M, int K, int R);

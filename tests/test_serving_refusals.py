@@ -90,3 +90,16 @@ def test_the_binding_refuses_tensors_off_the_gpu():
             call()
     with pytest.raises(ValueError):
         quant_hip.kv4_attention(q, cache, t, n, scale=-1.0)
+
+
+def test_sizes_beyond_what_a_launch_can_cover():
+    from alpaca_lora_4bit_amd import _lib
+    L = _lib.lib()
+    over = dict(T=2 ** 24 + 2)
+    assert L.q4_kv4_append_f16(*_args(**over), FAKE, 256, 128, FAKE, 256, 128, None, 0, 0, None, 0, None, 0, 0, 0, None) == -2
+    assert L.q4_kv4_read_f16(*_args(**over), FAKE, FAKE, None) == -2
+    assert L.q4_kv4_attention_f16(*_args(**over), FAKE, 256, 128, 2, 1.0, FAKE, 2, 64, FAKE, 1 << 30, None) == -2
+    assert L.q4_lora_rows_workspace_bytes(1, 2 ** 24 + 1, 256, 8) == 0 and L.q4_lora_rows_workspace_bytes(1, 2 ** 24, 256, 8) > 0
+    # bounds that are far too small for the rows do not ask for more than a gigabyte
+    for T, D in ((2 ** 20, 128), (2 ** 24, 64), (64, 128)):
+        assert L.q4_kv4_attention_workspace_bytes(*_args(T=T, D=D, width=2 ** 22), 64, 1, 2 ** 26) <= 2 ** 30
