@@ -86,10 +86,10 @@ __global__ __launch_bounds__(64 * kRowsWaves) void lora_rows_down_kernel(RowsArg
             const int col = ch * kRowsChunk + lc;
             const int at = ch < c1 && col < ra.K ? (lr * ra.K + col) * 2 : kRowsFar;      // what is not there comes as zero
 #pragma unroll
-            for (int i = 0; i < 4 * RB; ++i) v[i] = buf_load128(rs_a, at, 8 * i * ra.K);
+            for (int i = 0; i < 4 * RB; ++i) v[i] = buf_load128(rs_a, at + 8 * i * ra.K, 0);
 #pragma unroll
             for (int i = 0; i < 4 * MT; ++i)                               // four rows without this adapter: no traffic
-                v[4 * RB + i] = buf_load128(rs_x, at, mine >> (4 * i) & 15u ? 8 * i * ra.K : kRowsFar);
+                v[4 * RB + i] = buf_load128(rs_x, mine >> (4 * i) & 15u ? at + 8 * i * ra.K : kRowsFar, 0);
         };
         request(c0 + wave);
         for (int ch = c0 + wave; ch < c1; ch += kRowsWaves) {
@@ -240,13 +240,20 @@ __global__ __launch_bounds__(64 * kRowsWaves) void lora_rows_up_kernel(RowsArgs 
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             if (MT > 1 && !(mine >> (16 * t) & 0xFFFFu)) continue;
+            // the lane's row takes the products of its own adapter only: zeros times an infinity of another one would be no zeros
+            const bool own = mine >> (16 * t + r) & 1;
+            float4_t sum[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum[u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
                 half8_t xb = {};
-                if (mine >> (16 * t + r) & 1) xb = sx[16 * t + r][4 * i + kk];
+                if (own) xb = sx[16 * t + r][4 * i + kk];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[i % NS][u], xb, acc[t][u], 0, 0, 0);
+                for (int u = 0; u < 4; ++u) sum[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[i % NS][u], xb, sum[u], 0, 0, 0);
             }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[t][u] = own ? sum[u] : acc[t][u];
         }
     }
 #pragma unroll

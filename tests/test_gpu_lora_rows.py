@@ -84,3 +84,27 @@ def test_infinities_and_nan_stay_in_their_rows():
     bad = torch.zeros(M, dtype=torch.bool)
     bad[4], bad[5], bad[idx == 0] = True, True, True
     assert torch.equal(got[~bad.cuda()], want[~bad.cuda()]) and not torch.isfinite(got[bad.cuda()]).any()
+
+
+@pytest.mark.parametrize("M", [3, 40, 300])
+def test_an_adapter_that_is_no_number_stays_with_its_requests(M):
+    """Infinities and NaN in one adapter's matrices or scaling: its rows are no numbers, all others come out as without it."""
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip
+    rng = np.random.default_rng(M)
+    x = torch.from_numpy(rng.standard_normal((M, 256)).astype(np.float16)).cuda()
+    a = torch.from_numpy((rng.standard_normal((3, 16, 256)) / 16).astype(np.float16)).cuda()
+    b = torch.from_numpy(rng.standard_normal((3, 320, 16)).astype(np.float16)).cuda()
+    index = torch.from_numpy((np.arange(M) % 4 - 1).astype(np.int32)).cuda()
+    s, y0 = torch.ones(3, device="cuda"), torch.ones(M, 320, dtype=torch.float16, device="cuda")
+    want = y0.clone()
+    quant_hip.lora_rows(x, index, [(a, b, s, want)])
+    theirs = index == 1
+    for what in range(3):
+        for value in (float("nan"), float("inf")):
+            t = [a.clone(), b.clone(), s.clone()]
+            t[what].view(3, -1)[1] = value
+            y = y0.clone()
+            quant_hip.lora_rows(x, index, [(t[0], t[1], t[2], y)])
+            assert torch.equal(y[~theirs], want[~theirs])
+            assert not torch.isfinite(y[theirs]).all(dim=-1).any()
