@@ -727,9 +727,12 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4Attn a) {
 // ---- plan ----------------------------------------------------------------------------------------
 struct Kv4AttnPlan { bool prompt; int blocks, nsplit; };
 
-// Above 64 rows a key head and sequence the prompt kernel, below it 16 rows a workgroup.  The keys are split, a share of 256 keys (a tile per wavefront) at
-// least, until two prompts' workgroups or two of one sequence stand for every compute unit (131072 tokens of one: 31.9 us with 512 workgroups, 34.1 with 1024, 39.1
-// with 2048, for the shares are joined), eight of four sequences or more, whose lengths differ (32 of up to 16384: 101.7, 82.3 and 77.2 us).
+// Above 64 rows a key head and sequence the prompt kernel, below it 16 rows a workgroup.
+// Prompts: the keys are split into shares of 256 at least while no more than two workgroups stand for every compute unit, for the ones beyond would wait for all
+// (189 tokens at 7227, 8 key heads of 4: 46.4 us in eleven shares, 42.9 in ten).
+// Rows: the shares, of 256 keys at least (a tile per wavefront), make two workgroups of one sequence for every compute unit (131072 tokens of one: 31.9 us with 512
+// workgroups, 34.1 with 1024, 39.1 with 2048, for the shares are joined), eight of four sequences or more, whose lengths differ (32 of up to 16384: 101.7, 82.3 and
+// 77.2 us); where there are 1024 workgroups without, a share has 1024 keys at least (35 requests of 40 heads and up to 265 tokens: 38.7 us in two shares, 25.7 in one).
 inline Kv4AttnPlan plan_kv4_attn(int B, int heads, int D, int share, int T, int max_tokens, int max_length) {
     Kv4AttnPlan p;
     const long rows = (long)max_tokens * share;
@@ -737,10 +740,10 @@ inline Kv4AttnPlan plan_kv4_attn(int B, int heads, int D, int share, int T, int 
     const int per = p.prompt ? kPromptRows : 16;
     p.blocks = (int)((rows + per - 1) / per);
     const long groups = (long)B * heads * p.blocks, wanted = p.prompt ? 512 : std::min(512l * B, 2048l);
-    const long most = std::max(1l, (max_length + 255l) / 256);
+    const long keys = !p.prompt && groups >= 1024 ? 1024 : 256, most = std::max(1l, (max_length + keys - 1) / keys);
     // bounds that are right ask for 200 MB at most; others must not ask for all memory, nor for more rows than the join can be launched for
     const long room = (1l << 30) / ((long)T * heads * share * (D + 2) * (long)sizeof(float));
-    p.nsplit = (int)std::max(1l, std::min({most, (wanted + groups - 1) / groups, 256l, room}));
+    p.nsplit = (int)std::max(1l, std::min({most, (p.prompt ? wanted : wanted + groups - 1) / groups, 256l, room}));
     return p;
 }
 
