@@ -218,8 +218,8 @@ def generate_batch(model, prompts, max_new_tokens, bank=None, adapters=None, eos
         raise ValueError("`bank` and `adapters` (one number for each prompt) go together")
     if adapters is not None and any(not -1 <= a < bank.count for a in adapters):
         raise ValueError(f"adapters must be -1 .. {bank.count - 1}")
-    if prefill_rows < 1:
-        raise ValueError("prefill_rows must be positive")
+    if prefill_rows < 1 or page < 1:
+        raise ValueError("prefill_rows and page must be positive")
     heads, kv_heads, head_dim = _attention_shape(model.config)
     dev = prompts[0].device
     totals = [p.numel() + max_new_tokens for p in prompts]

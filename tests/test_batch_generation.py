@@ -144,7 +144,7 @@ def test_generate_batch_refuses(monkeypatch):
     model = _model()
     bank = models.AdapterBank(model, _adapters(model, [("q_proj",)], (8,), 1), device="cpu")
     for kw in (dict(bank=bank), dict(adapters=[0]), dict(bank=bank, adapters=[0, 0]), dict(bank=bank, adapters=[1]), dict(bank=bank, adapters=[-2]),
-               dict(prefill_rows=0), dict(page=24), dict(group=128), dict(group=16)):
+               dict(prefill_rows=0), dict(page=0), dict(page=24), dict(group=128), dict(group=16)):
         with pytest.raises(ValueError):
             inference.generate_batch(model, [PROMPTS[0]], 2, use_graph=False, **kw)
     for prompts in ([PROMPTS[0][None]], [PROMPTS[0][:0]]):

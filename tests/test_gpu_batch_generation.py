@@ -126,6 +126,16 @@ def test_captured_steps_give_the_eager_tokens(tmp_path, oracle, adapters):
         assert base != want
 
 
+def test_prompts_in_small_parts(tmp_path, oracle):
+    """Parts in which no prompt ends, one row at a time at the least; the same parts give the same tokens."""
+    from alpaca_lora_4bit_amd import inference
+    build(str(tmp_path), oracle, seed=8)
+    model, _ = _loaded(str(tmp_path))
+    for rows in (1, 7):
+        got = [[t.tolist() for t in inference.generate_batch(model, _prompts()[:3], 3, prefill_rows=rows, page=32, group=64)] for _ in range(2)]
+        assert got[0] == got[1] and [len(g) for g in got[0]] == [len(p) + 3 for p in _prompts()[:3]]
+
+
 def test_requests_from_the_command_line(tmp_path, oracle):
     from safetensors.torch import save_file
     from alpaca_lora_4bit_amd import inference
