@@ -738,7 +738,7 @@ inline Kv4AttnPlan plan_kv4_attn(int B, int heads, int D, int share, int T, int 
     const long rows = (long)max_tokens * share;
     p.prompt = rows > 64;
     const int per = p.prompt ? kPromptRows : 16;
-    p.blocks = (int)((rows + per - 1) / per);
+    p.blocks = (int)std::max(1l, std::min((rows + per - 1) / per, (1l << 22) / ((long)B * heads)));   // a workgroup takes several where a launch has no room
     const long groups = (long)B * heads * p.blocks, wanted = p.prompt ? 512 : std::min(512l * B, 2048l);
     const long keys = !p.prompt && groups >= 1024 ? 1024 : 256, most = std::max(1l, (max_length + keys - 1) / keys);
     // bounds that are right ask for 200 MB at most; others must not ask for all memory, nor for more rows than the join can be launched for

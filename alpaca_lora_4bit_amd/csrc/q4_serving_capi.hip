@@ -32,8 +32,7 @@ bool heads_fit(const q4_kv4_cache_t* c, const q4_kv4_batch_t* b, int q_heads) {
 }
 bool launch_fits(const q4_kv4_cache_t* c, const q4_kv4_batch_t* b, int q_heads, int max_tokens, int max_length) {
     if (!heads_fit(c, b, q_heads) || max_tokens < 1 || max_length < 1) return false;
-    // workgroups before the keys are split; a split at most doubles the launch's 1024
-    return ((double)max_tokens * (q_heads / c->heads) / 16 + 1) * b->B * c->heads < 1073741824.0;
+    return (double)b->B * c->heads <= 4194304.0;                           // workgroups of one block of rows each, 2^32 threads a launch
 }
 bool strides_fit(long long t, long long h) { return t >= 0 && h >= 0 && t < (1ll << 40) && h < (1ll << 40); }
 bool vectors(const void* p, long long t, long long h) { return !misaligned(p) && t % 8 == 0 && h % 8 == 0; }
@@ -106,6 +105,7 @@ extern "C" int q4_lora_rows_f16(const q4_lora_rows_t* probs, int count, const vo
         const q4_lora_rows_t& g = probs[i];
         if (!g.a || !g.b || !g.scaling || !g.y) return Q4_ERR_NULL_POINTER;
         if (g.N < 64 || g.N % 64 != 0 || g.N > (1 << 23)) return Q4_ERR_BAD_SHAPE;
+        if (((M + 31ll) / 32) * ((g.N + 255) / 256) >= (1 << 24)) return Q4_ERR_BAD_SHAPE;      /* 2^32 threads a launch */
         if (misaligned(g.a) || misaligned(g.b) || misaligned(g.y)) return Q4_ERR_MISALIGNED;
     }
     if (!workspace || workspace_bytes < q4_lora_rows_workspace_bytes(count, M, K, R)) return Q4_ERR_WORKSPACE;

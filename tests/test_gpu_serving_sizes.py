@@ -85,3 +85,22 @@ def test_many_query_heads_on_one_key_head(new):
     want, tol = o.attention(q, cache, table, np.array([130, 5]), None, 0.125, new * 48 > 64)
     got = quant_hip.kv4_attention(_cuda(q), tuple(_cuda(c) for c in cache), _cuda(table), torch.tensor([130, 5], dtype=torch.int32).cuda())
     _check(got, want, tol)
+
+
+def test_more_blocks_of_rows_than_a_launch_has_workgroups():
+    """Twenty thousand sequences of one row each without a bound on their rows: the launch is sized for all rows in one sequence and has to take them in turns."""
+    import torch
+    from alpaca_lora_4bit_amd import kv4_cache, quant_hip
+    B = 20000
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    half = lambda *s: torch.randn(*s, generator=gen, device="cuda").half()
+    cache = kv4_cache.new_layer(B, 4, 64, 16, 64)
+    table = torch.randperm(B, generator=gen, device="cuda").int().view(B, 1)
+    for n in (1, 2):
+        quant_hip.kv4_append(half(B, 4, 64), half(B, 4, 64), cache, table, torch.full((B,), n, dtype=torch.int32, device="cuda"))
+    lengths, starts = torch.full((B,), 2, dtype=torch.int32, device="cuda"), torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    q = half(B, 8, 64)
+    want = quant_hip.kv4_attention(q, cache, table, lengths, starts=starts, max_tokens=1)
+    got = quant_hip.kv4_attention(q, cache, table, lengths, starts=starts)
+    # two weights and two values, each rounded once more (2^-11 of values up to 6), and the results (2^-11)
+    assert float((got.float() - want.float()).abs().max()) <= 4 * 6 * 2 ** -11

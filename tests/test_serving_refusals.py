@@ -103,3 +103,9 @@ def test_sizes_beyond_what_a_launch_can_cover():
     # bounds that are far too small for the rows do not ask for more than a gigabyte
     for T, D in ((2 ** 20, 128), (2 ** 24, 64), (64, 128)):
         assert L.q4_kv4_attention_workspace_bytes(*_args(T=T, D=D, width=2 ** 22), 64, 1, 2 ** 26) <= 2 ** 30
+    many = dict(B=2 ** 12, T=2 ** 12, heads=2048, pages=4)
+    assert L.q4_kv4_attention_f16(*_args(**many), FAKE, 2 ** 19, 128, 2048, 1.0, FAKE, 1, 64, FAKE, 1 << 30, None) == -2
+    p = (_lib.LoraRows * 4)()
+    p[0].a = p[0].b = p[0].scaling = p[0].y = FAKE
+    p[0].N = 2 ** 13 + 64
+    assert L.q4_lora_rows_f16(p, 1, FAKE, FAKE, 1, 2 ** 24, 32, 8, 1, FAKE, 1 << 40, None) == -2
