@@ -9,6 +9,7 @@
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -862,7 +863,7 @@ void lora_rows(const at::Tensor& x, const at::Tensor& index, const std::vector<R
     check_no_grad(x, "x");
     const int64_t M = x.size(0), K = x.size(1);
     TORCH_CHECK_VALUE(per >= 1 && index.scalar_type() == at::kInt && index.dim() == 1 && index.is_contiguous() && index.device() == x.device() &&
-                      index.size(0) == (M + per - 1) / per, "index must be a contiguous int32 tensor on x's device, one entry for each ", per, " rows");
+                      index.size(0) == (M == 0 ? 0 : (M - 1) / per + 1), "index must be a contiguous int32 tensor on x's device, one entry for each ", per, " rows");
     q4_lora_rows_t probs[4];
     int64_t n = 0, R = 0;
     for (size_t i = 0; i < count; ++i) {
@@ -893,10 +894,11 @@ void lora_rows(const at::Tensor& x, const at::Tensor& index, const std::vector<R
     TORCH_CHECK_VALUE(K >= 32 && K % 32 == 0 && K <= (1 << 20) && M <= (1 << 24), "K must be a multiple of 32 up to 2^20, and x have up to 2^24 rows");
     TORCH_CHECK_VALUE(n < (1ll << 31) && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, "x must be 16-byte aligned");
     if (M == 0 || n == 0) return;
+    const int run = (int)std::min(per, M);                     // 32 bits hold it: a run longer than x is all of x
     Launch L(x.device());
     const size_t need = q4_lora_rows_workspace_bytes((int)count, (int)M, (int)K, (int)R);
     const at::Tensor ws = at::empty({(int64_t)need}, x.options().dtype(at::kByte));
-    const int rc = q4_lora_rows_f16(probs, (int)count, x.data_ptr(), index.data_ptr<int>(), (int)per, (int)M, (int)K, (int)R, (int)n, ws.data_ptr(), need,
+    const int rc = q4_lora_rows_f16(probs, (int)count, x.data_ptr(), index.data_ptr<int>(), run, (int)M, (int)K, (int)R, (int)n, ws.data_ptr(), need,
                                     L.stream);
     if (rc != Q4_OK) raise_q4(rc, "q4_lora_rows_f16");
 }
