@@ -1,6 +1,6 @@
 // Appending to the 4-bit key/value cache (layout in q4_kv4.hpp) and reading places of it back.
 //
-//   append:  k' = R(pos) k,  scale = rn16(max|k'| / 6) over a group,  code = nearest(k' / scale);  v likewise without R;  q' = R(pos) q
+//   append:  k' = R(pos) k,  scale = rn16(max|k'| / 6) over a group (10912 at most where that fits fp16),  code = nearest(k' / scale);  v likewise without R;  q' = R(pos) q
 //   read:    rn16(code * scale)
 //
 // R turns the first `rot` dimensions by pairs, (x_i, x_{i + rot/2}) or (x_{2i}, x_{2i+1}), with cosine and sine from a float32 table
@@ -77,7 +77,11 @@ __device__ __forceinline__ void kv4_turned8(const Kv4Turn& r, const half_t* row,
 
 // Magnitudes are compared as integers: an infinity or a NaN among them is the largest and reaches the scale.
 __device__ __forceinline__ uint32_t kv4_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
-__device__ __forceinline__ half_t kv4_scale(uint32_t bits) { return (half_t)(__builtin_bit_cast(float, bits) / 6.0f); }
+// A group that fits fp16 has a scale of 10912 at most: 65504 / 6 rounds up to 10920, whose sixfold is none of fp16's numbers.
+__device__ __forceinline__ half_t kv4_scale(uint32_t bits) {
+    const float x = __builtin_bit_cast(float, bits), s = x / 6.0f;
+    return (half_t)(x <= 65504.0f ? fminf(s, 10912.0f) : s);
+}
 __device__ __forceinline__ float kv4_over(float x, float scale) { return scale > 0.0f ? x / scale : 0.0f; }
 
 template <int D, int NG, bool VEC>

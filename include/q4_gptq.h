@@ -368,7 +368,8 @@ Q4_API int q4_lora_grad_grouped_f32(const q4_lora_grad_t *probs, int n, int M, i
 
 /* ---- serving many requests at once ------------------------------------------------------------------------------------
  * A paged cache of keys and values in 4 bits.  A value is code * scale: codes are 4-bit floats (1 sign, 2 exponent, 1 mantissa
- * bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), scales fp16 = largest magnitude / 6 of `group` dimensions of one token and head.  With NG = D / group:
+ * bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), scales fp16 = largest magnitude / 6 of `group` dimensions of one token and head (10912 at most where the
+ * group fits fp16: 6 * 10920, what 65504 / 6 rounds to, would not).  With NG = D / group:
  *   k_codes  int32 [pages, heads, page, D/8]       word kk*(D/32) + s (kk < 4) of a token: dimensions 32*s + 8*kk .. + 7, lowest nibble first
  *   v_codes  int32 [pages, heads, page/4, D/8, 4]  word j of four tokens side by side; with H = D/16, nibble i + H*r is dimension 16*i + (D/8)*r + j
  *   k_scales, v_scales  fp16 [pages, heads, NG, page]

@@ -38,10 +38,12 @@ def encode(y):
 
 
 def quantize(x, group):
-    """(codes, scales) of float32 x [..., D]."""
+    """(codes, scales) of float32 x [..., D]; a group that fits fp16 has a scale of 10912 at most, whose largest code does."""
     g = x.astype(np.float32).reshape(*x.shape[:-1], -1, group)
     with np.errstate(over="ignore"):
-        scales = (np.abs(g).max(-1) / np.float32(6.0)).astype(np.float16)
+        top = np.abs(g).max(-1)
+        scales = (top / np.float32(6.0)).astype(np.float16)
+    scales = np.where(top <= 65504, np.minimum(scales, np.float16(10912)), scales)
     s = scales.astype(np.float32)[..., None]
     with np.errstate(divide="ignore", invalid="ignore"):
         y = np.where(s > 0, g / s, np.float32(0))

@@ -1,0 +1,45 @@
+"""Values and keys at the top of fp16's range and beyond it: what append makes of the largest numbers, scales that a cache of the caller's own holds, keys that a rotation took
+above fp16, and that no finite number of a later token reaches the rows before it."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_kv4 import _check, _cuda, _filled
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("D,group", [(128, 128), (128, 32), (64, 64)])
+def test_the_largest_numbers_come_back_finite(D, group):
+    """Groups whose largest magnitude is fp16's largest number or one of the next below it: what is stored stays inside fp16's range, off by a 4-bit step at most, and
+    attention over it is finite for one row and for many."""
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip
+    from oracle import kv4_oracle as o
+    rng = np.random.default_rng(D + group)
+    n, tops = 70, [65504.0, -65504.0, 65472.0, -65440.0, 65408.0]
+    k, v = (rng.standard_normal((n, 1, D)).astype(np.float16) * np.float16(1000) for _ in range(2))
+    for i in range(n):
+        for x in (k, v):
+            x[i, 0, rng.integers(group):: group] = tops[i % 5]
+    want = o.new_cache(5, 1, 16, D, group)
+    table = np.arange(5, dtype=np.int32)[None]
+    for i in range(n):
+        (kq, ks), (vq, vs) = o.quantize(k[i, 0].astype(np.float32), group), o.quantize(v[i, 0].astype(np.float32), group)
+        assert max(ks.max(), vs.max()) <= 10912
+        o.put(want, i // 16, 0, i % 16, kq, ks, vq, vs)
+    cache = tuple(_cuda(x) for x in o.new_cache(5, 1, 16, D, group))
+    args = (cache, _cuda(table), torch.tensor([n], dtype=torch.int32).cuda())
+    quant_hip.kv4_append(_cuda(k), _cuda(v), *args)
+    for got, w in zip(cache, want):
+        assert np.array_equal(got.cpu().numpy(), w, equal_nan=w.dtype == np.float16)
+    for got, x in zip(quant_hip.kv4_read(*args, n), (k, v)):
+        got = got.float().cpu().numpy()
+        # half a step between 4 and 6 of a scale of 10912; the largest number itself is 32 off
+        assert np.isfinite(got).all() and np.abs(got - x.astype(np.float32)).max() <= 10912
+        assert (np.abs(got - x.astype(np.float32))[np.abs(x.astype(np.float32)) > 60000] <= 32).all()
+    for rows in (1, n):
+        q = (rng.standard_normal((rows, 1, D)) * 1e-4).astype(np.float16)
+        ref, tol = o.attention(q, want, table, np.array([n]), None, 1 / math.sqrt(D), rows > 64)
+        _check(quant_hip.kv4_attention(_cuda(q), *args), ref, tol, rows)
