@@ -98,10 +98,10 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4Cache& c, const Kv4Batch&
     return r;
 }
 
-// two of the four code bytes' values: byte SEL of w, low nibble first
+// two of the four code bytes' values, times `factor`, a power of two: byte SEL of w, low nibble first
 template <int SEL>
-__device__ __forceinline__ half2_t kv4_pair(uint32_t w) {
-    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, SEL);
+__device__ __forceinline__ half2_t kv4_pair(uint32_t w, float factor = 1.0f) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, factor, SEL);
 }
 __device__ __forceinline__ half8_t kv4_word(uint32_t w) {
     const uint4_t x = {as_u32(kv4_pair<0>(w)), as_u32(kv4_pair<1>(w)), as_u32(kv4_pair<2>(w)), as_u32(kv4_pair<3>(w))};

@@ -44,6 +44,7 @@ __device__ __forceinline__ float max_of_halves(float x) {
 typedef float float2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t rounded_pair(float a, float b) { return as_u32(__builtin_convertvector(float2_t{a, b}, half2_t)); }
 
+__device__ __forceinline__ uint32_t magnitude_bits(half_t x) { return __builtin_bit_cast(uint16_t, x) & 0x7FFFu; }
 __device__ __forceinline__ bool finite_bits(half_t x) { return (__builtin_bit_cast(uint16_t, x) & 0x7C00u) != 0x7C00u; }
 
 typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(256, 3) void kv4_attn_rows_kernel(Kv4Attn a) {
                 for (int i = 0; i < 16 * NG; ++i) {
                     const half_t x = scales[wave][1][i >> 4][16 * kk + (i & 15)];
                     if ((i & 15) < seen) {
-                        if (finite_bits(x)) big = fmaxf(big, (float)x);
+                        if (finite_bits(x)) big = fmaxf(big, fabsf((float)x));
                         else l = NAN;
                     }
                 }
@@ -333,6 +334,12 @@ __global__ __launch_bounds__(256, 3) void kv4_attn_rows_kernel(Kv4Attn a) {
 // last block's 32 tiles are 55; parts of four prompts (509, 434, 360, 286 tokens at 8191, 5062, 1933, 6995; 8 key heads of 4): 195 us, 128 tiles one after the other.
 // Eight wavefronts on 256 rows, half turning keys, half values: 69 and 216 us, for all are at the same step; splitting the keys of whole prompts costs the join more
 // than the balance gives (parts: 271 us in two shares).
+//
+// Values beyond fp16 (a scale above 10912, whose sixfold passes it; append writes none) would be infinite in LDS, and nothing times infinity is no number
+// for the rows that do not see them.  The staging finds such a scale, and the rows are gone through a second time with an eighth of every value, which holds all of them.
+constexpr uint32_t kMostValueScale = 0x7154u;          // 10912 in fp16
+constexpr uint32_t kAboveMost = (0x7FFFu - kMostValueScale) * 0x10001u;      // added to two magnitudes: the sign of one that is greater
+constexpr float kLessen = 0.125f;
 constexpr float kSlack = 5.0f;
 constexpr int kPromptRows = 128;
 constexpr int kFewKeys = 1024;
@@ -350,6 +357,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
     __shared__ __attribute__((aligned(16))) Kv4Staged<D> tiles_lds[2];
     __shared__ __attribute__((aligned(16))) float key_scales[2][NG][64];
     __shared__ int poison;                                                 // first key seen whose values are no numbers
+    __shared__ int large;                                                  // whether a value seen is beyond fp16
     __shared__ int there[2][4];                                            // whether the tile's runs of 16 keys lie on pages of the cache
     const int lane = threadIdx.x & 63, r = lane & 31, h32 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -383,7 +391,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
     const int* table = a.p.table + (size_t)b * a.p.width;
     const int rows = n * a.share;
 
-    for (int row0 = block0 * kPromptRows; row0 < rows; row0 += a.blocks * kPromptRows) {
+    float lessen = 1.f;                                                    // of the values; kLessen while rows are gone through a second time
+    for (int row0 = block0 * kPromptRows; row0 < rows;) {
         const int row = row0 + 32 * wave + r;
         const int tok = first + row / a.share, qh = h * a.share + row % a.share;
         const bool live = row < rows && tok >= 0 && tok < a.p.T;
@@ -393,7 +402,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
         const int kend = max(0, min(len - n + min(row0 + kPromptRows - 1, rows - 1) / a.share + 1, cap));
         const int tiles = (kend + 63) / 64, per = (tiles + a.nsplit - 1) / a.nsplit;
         const int t0 = split * per, t_end = min(t0 + per, tiles);
-        if (threadIdx.x == 0) poison = 0x7FFFFFFF;
+        if (threadIdx.x == 0) { poison = 0x7FFFFFFF; large = 0; }
 
         half8_t qf[ST];
 #pragma unroll
@@ -454,15 +463,16 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
         auto look = [&](Raw& x, int buf, int tile) __attribute__((always_inline)) {
             const int key = tile * 64 + 16 * wave;
             there[buf][wave] = x.have | -(int)(key >= kend);
-            uint32_t odd = 0;                                              // the sign of a half: an exponent of all ones
+            uint32_t odd = 0;                                              // the sign of a half: a magnitude above kMostValueScale, or no number
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const uint2_t w = __builtin_bit_cast(uint2_t, x.vs[g]);
-                odd |= ((w.x & 0x7C007C00u) + 0x04000400u) | ((w.y & 0x7C007C00u) + 0x04000400u);
+                odd |= ((w.x & 0x7FFF7FFFu) + kAboveMost) | ((w.y & 0x7FFF7FFFu) + kAboveMost);
             }
             if (__builtin_expect((key + 16 <= kend) & (__ballot((odd & 0x80008000u) != 0) == 0) & (x.have != 0), 1)) return;
             const int ks_in = x.have ? kend - key - kc : 0, vs_in = x.have ? kend - key - 4 * kk : 0;
             int strange = 0x7FFFFFFF;
+            uint32_t most = 0;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 if (ks_in <= 0) x.ks[g] = (half_t)0.f;
@@ -471,9 +481,11 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
                     const bool finite = finite_bits(x.vs[g][e]);
                     if (e < vs_in && !finite) strange = min(strange, key + 4 * kk + e);
                     if (e >= vs_in || !finite) x.vs[g][e] = (half_t)0.f;
+                    most = max(most, magnitude_bits(x.vs[g][e]));
                 }
             }
             if (__any(strange != 0x7FFFFFFF)) atomicMin(&poison, strange);
+            if (__any(most > kMostValueScale)) large = 1;
         };
         const int kb_w = wave >> 1;                                        // the half of a tile that this wavefront's keys lie in
         const int kr_w = 16 * (wave & 1) + kc;
@@ -508,7 +520,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
             for (int q = 0; q < 2; ++q) {
                 const uint32_t w = pr[q][i & 1];
                 const half2_t f = {x.vs[i / HG][2 * q], x.vs[i / HG][2 * q + 1]};
-                const half2_t d = i / 2 == 0 ? kv4_pair<0>(w) : i / 2 == 1 ? kv4_pair<1>(w) : i / 2 == 2 ? kv4_pair<2>(w) : kv4_pair<3>(w);
+                const half2_t d = i / 2 == 0 ? kv4_pair<0>(w, lessen) : i / 2 == 1 ? kv4_pair<1>(w, lessen) : i / 2 == 2 ? kv4_pair<2>(w, lessen) : kv4_pair<3>(w, lessen);
                 y[q] = as_u32(d * f);
             }
             uint4_t* at = &tiles_lds[buf].v[((kb_w * 2 + (wave & 1)) * DB + i / 2) * 64 + 32 * (kk & 1) + 16 * (i & 1) + c];
@@ -635,6 +647,11 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
         };
         if (kend <= kFewKeys) all(std::true_type{});
         else all(std::false_type{});
+        if (__builtin_expect((large != 0) & (lessen == 1.f), 0)) {            // the same for all: the last write to it lies before the last barrier
+            lessen = kLessen;
+            __syncthreads();
+            continue;
+        }
         if (limit > poison) l = NAN;
         {
             const uint32_t lb = __builtin_bit_cast(uint32_t, l);
@@ -644,7 +661,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
         }
         if (live) {                                                        // o[i][e]: dimension 32*i + 8*(e/4) + 4*h32 + e%4
             const size_t at = (size_t)tok * a.hq + qh, all = (size_t)a.p.T * a.hq;
-            const float f = l == 0.f ? 0.f : 1.f / l;
+            const float up = 1.f / lessen, f = l == 0.f ? 0.f : up / l;
 #pragma unroll
             for (int i = 0; i < DB; ++i)
 #pragma unroll
@@ -658,7 +675,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
                     } else {
                         float4_t y;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) y[e] = o[i][4 * q + e];
+                        for (int e = 0; e < 4; ++e) y[e] = o[i][4 * q + e] * up;
                         *reinterpret_cast<float4_t*>(a.part + (split * all + at) * D + d) = y;
                     }
                 }
@@ -668,6 +685,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
                 ml[1] = l;
             }
         }
+        row0 += a.blocks * kPromptRows;
+        lessen = 1.f;
         __syncthreads();
     }
 }

@@ -43,3 +43,23 @@ def test_the_largest_numbers_come_back_finite(D, group):
         q = (rng.standard_normal((rows, 1, D)) * 1e-4).astype(np.float16)
         ref, tol = o.attention(q, want, table, np.array([n]), None, 1 / math.sqrt(D), rows > 64)
         _check(quant_hip.kv4_attention(_cuda(q), *args), ref, tol, rows)
+
+
+
+@pytest.mark.parametrize("scale", [10920.0, 20000.0, -65504.0])
+@pytest.mark.parametrize("D,group,length,new", [(128, 128, 200, 200), (128, 32, 300, 130), (64, 64, 1300, 150), (64, 32, 150, 150), (128, 64, 80, 2)])
+def test_finite_values_of_any_scale_count_for_the_rows_that_see_them_only(D, group, length, new, scale):
+    """A value of code 6 at these scales passes fp16.  Rows that see it get it, those before it are as the formula has them."""
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip
+    from oracle import kv4_oracle as o
+    rng = np.random.default_rng(length + new)
+    cache, table = _filled(o, [length], 1, D, group, 48, rng)
+    at = length - new + new // 2
+    cache[3][table[0, at // 48], 0, -1, at % 48] = scale
+    q = (rng.standard_normal((new, 1, D)) * 0.3).astype(np.float16)
+    want, tol = o.attention(q, cache, table, np.array([length]), None, 1 / math.sqrt(D), new > 64)
+    assert np.abs(want).max() < 60000
+    args = (tuple(_cuda(x) for x in cache), _cuda(table), torch.tensor([length], dtype=torch.int32).cuda())
+    for bounds in (dict(max_length=64), dict(max_tokens=new, max_length=5000)):
+        _check(quant_hip.kv4_attention(_cuda(q), *args, **bounds), want, tol, bounds)
