@@ -56,7 +56,7 @@ struct Kv4Attn {
     long q_t, q_h;
     half_t* out;              // [T, hq, D]
     float* part;              // [nsplit][T * hq][D] sums, then [nsplit][T * hq][2] maxima and sums of weights; null: nsplit 1
-    float scale;              // softmax scale * log2(e)
+    float scale, scale8;      // softmax scale * log2(e), and eight times that
     int hq, share, nsplit, blocks;    // share = hq / heads; row blocks in the grid
     uint32_t page_magic;      // ceil(2^32 / (page / 16)), 0 for pages of 16
 };

@@ -337,6 +337,8 @@ __global__ __launch_bounds__(256, 3) void kv4_attn_rows_kernel(Kv4Attn a) {
 //
 // Values beyond fp16 (a scale above 10912, whose sixfold passes it; append writes none) would be infinite in LDS, and nothing times infinity is no number
 // for the rows that do not see them.  The staging finds such a scale, and the rows are gone through a second time with an eighth of every value, which holds all of them.
+// Rounded keys are eighths always (a rotation takes pairs of large numbers beyond fp16; the conversion from codes multiplies by a power of two for nothing), and the softmax
+// scale is eightfold; keys below 2^-11 lose up to three bits by it.
 constexpr uint32_t kMostValueScale = 0x7154u;          // 10912 in fp16
 constexpr uint32_t kAboveMost = (0x7FFFu - kMostValueScale) * 0x10001u;      // added to two magnitudes: the sign of one that is greater
 constexpr float kLessen = 0.125f;
@@ -496,7 +498,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
                 if (s % SG == 0) key_scales[buf][s / SG][16 * wave + kc] = (float)x.ks[s / SG];
             } else {
                 const half2_t f = {x.ks[s / SG], x.ks[s / SG]};
-                y = uint4_t{as_u32(kv4_pair<0>(x.k[s]) * f), as_u32(kv4_pair<1>(x.k[s]) * f), as_u32(kv4_pair<2>(x.k[s]) * f), as_u32(kv4_pair<3>(x.k[s]) * f)};
+                y = uint4_t{as_u32(kv4_pair<0>(x.k[s], kLessen) * f), as_u32(kv4_pair<1>(x.k[s], kLessen) * f), as_u32(kv4_pair<2>(x.k[s], kLessen) * f),
+                            as_u32(kv4_pair<3>(x.k[s], kLessen) * f)};
             }
             tiles_lds[buf].k[((kb_w * ST + 2 * s) * 2 + kq) * kHalfPiece + kr_w] = y;
         };
@@ -577,10 +580,11 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
                         s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) < until ? s[kb][e] : -INFINITY;
                     }
             }
+            const float scale = EXACT ? a.scale : a.scale8;
             float mx = s[0][0];
 #pragma unroll
             for (int e = 1; e < 32; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
-            mx = max_of_halves(mx) * a.scale;
+            mx = max_of_halves(mx) * scale;
             if (__builtin_expect(__any(mx > m + kSlack), 0)) {
                 const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
                 l *= f;
@@ -594,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
                 float p[2];
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
-                    p[d] = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][(e & 15) + d], a.scale, base));
+                    p[d] = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][(e & 15) + d], scale, base));
                     l += p[d];
                 }
                 pw[e >> 3][(e & 7) >> 1] = rounded_pair(p[0], p[1]);
@@ -784,6 +788,7 @@ static void launch_attn(const q4::Kv4Attn& a, bool prompt, hipStream_t stream) {
 
 int q4_launch_kv4_attn(q4::Kv4Attn& a, int D, int group, int max_tokens, int max_length, hipStream_t stream) {
     const q4::Kv4AttnPlan p = q4::plan_kv4_attn(a.p.B, a.c.heads, D, a.share, a.p.T, max_tokens, max_length);
+    a.scale8 = a.scale * (1.f / q4::kLessen);
     a.blocks = p.blocks;
     a.nsplit = p.nsplit;
     const uint32_t p16 = a.c.page / 16;

@@ -77,13 +77,13 @@ extern "C" int q4_kv4_attention_f16(const q4_kv4_cache_t* cache, const q4_kv4_ba
     if (rc != Q4_OK) return rc;
     if (!q || !out) return Q4_ERR_NULL_POINTER;
     if (!launch_fits(cache, batch, q_heads, max_tokens, max_length) || !strides_fit(q_t, q_h)) return Q4_ERR_BAD_SHAPE;
-    if (!(scale > 0.0f) || !(scale < 3e38f)) return Q4_ERR_BAD_SHAPE;
+    if (!(scale > 0.0f) || !(scale < 1e37f)) return Q4_ERR_BAD_SHAPE;       // times 8 * log2(e) it is finite
     if (!vectors(q, q_t, q_h) || misaligned(out)) return Q4_ERR_MISALIGNED;
     const size_t need = q4_kv4_attention_workspace_bytes(cache, batch, q_heads, max_tokens, max_length);
     if (need && (!workspace || workspace_bytes < need)) return Q4_ERR_WORKSPACE;
     if (need && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return Q4_ERR_MISALIGNED;
     q4::Kv4Attn a{cache_of(cache), batch_of(batch), reinterpret_cast<const q4::half_t*>(q), (long)q_t, (long)q_h,
-                  reinterpret_cast<q4::half_t*>(out), reinterpret_cast<float*>(workspace), scale * 1.4426950408889634f, q_heads,
+                  reinterpret_cast<q4::half_t*>(out), reinterpret_cast<float*>(workspace), scale * 1.4426950408889634f, 0.f, q_heads,
                   q_heads / cache->heads, 1, 1, 0u};
     return q4_launch_kv4_attn(a, cache->D, cache->group, max_tokens, max_length, (hipStream_t)stream);
 }

@@ -63,3 +63,21 @@ def test_finite_values_of_any_scale_count_for_the_rows_that_see_them_only(D, gro
     args = (tuple(_cuda(x) for x in cache), _cuda(table), torch.tensor([length], dtype=torch.int32).cuda())
     for bounds in (dict(max_length=64), dict(max_tokens=new, max_length=5000)):
         _check(quant_hip.kv4_attention(_cuda(q), *args, **bounds), want, tol, bounds)
+
+
+@pytest.mark.parametrize("scale", [11784.0, 15448.0, -65504.0])
+@pytest.mark.parametrize("D,group,length,new", [(128, 128, 1100, 100), (64, 32, 1300, 400), (128, 32, 300, 100), (64, 64, 1100, 1)])
+def test_keys_of_any_finite_scale_give_finite_scores(D, group, length, new, scale):
+    """Two coordinates of 50000 that a rotation turns into one of 70711: finite scores whether a row sees few keys or more than a thousand."""
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip
+    from oracle import kv4_oracle as o
+    rng = np.random.default_rng(length + new)
+    cache, table = _filled(o, [length], 1, D, group, 48, rng)
+    for at in (3, length - new // 2 - 1):
+        cache[2][table[0, at // 48], 0, 0, at % 48] = scale
+    q = (rng.standard_normal((new, 1, D)) / abs(scale)).astype(np.float16)
+    want, tol = o.attention(q, cache, table, np.array([length]), None, 1 / math.sqrt(D), new > 64)
+    args = (tuple(_cuda(x) for x in cache), _cuda(table), torch.tensor([length], dtype=torch.int32).cuda())
+    for bounds in (dict(max_length=64), dict(max_tokens=new, max_length=5000)):
+        _check(quant_hip.kv4_attention(_cuda(q), *args, **bounds), want, tol, bounds)
