@@ -61,6 +61,9 @@ struct Kv4Attn {
     uint32_t page_magic;      // ceil(2^32 / (page / 16)), 0 for pages of 16
 };
 
+// A sequence's length, so far inside 32 bits that a batch's rows can be added and taken away: at most 2^26 places and 2^24 rows can matter.
+__device__ __forceinline__ int kv4_length(const Kv4Batch& p, int b) { return min(max(p.lengths[b], -(1 << 25)), 1 << 28); }
+
 struct Kv4Place {
     int pos, page, off;       // position in the sequence, page and offset in it
     bool mine, ok;            // the row belongs to a sequence; it has a place in the cache
@@ -90,7 +93,7 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4Cache& c, const Kv4Batch&
         r.mine = t >= first;
     }
     if (!r.mine) return r;
-    r.pos = p.lengths[b] - end + t;
+    r.pos = kv4_length(p, b) - end + t;
     if (r.pos < 0 || r.pos / c.page >= p.width) return r;
     r.page = p.table[(size_t)b * p.width + r.pos / c.page];
     r.off = r.pos % c.page;

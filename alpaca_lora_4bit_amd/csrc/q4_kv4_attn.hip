@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256, 3) void kv4_attn_rows_kernel(Kv4Attn a) {
     const int b = id / a.blocks;
     const int first = a.p.starts ? a.p.starts[b] : b * (a.p.T / a.p.B);
     const int n = min((a.p.starts ? a.p.starts[b + 1] : (b + 1) * (a.p.T / a.p.B)) - first, a.p.T);
-    const int len = a.p.lengths[b], cap = a.p.width * a.c.page, p16 = a.c.page / 16;
+    const int len = kv4_length(a.p, b), cap = a.p.width * a.c.page, p16 = a.c.page / 16;
     const int* table = a.p.table + (size_t)b * a.p.width;
     const int rows = n * a.share;
 
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_prompt_kernel(Kv4Attn a) {
     }
     const int first = a.p.starts ? a.p.starts[b] : b * (a.p.T / a.p.B);
     const int n = min((a.p.starts ? a.p.starts[b + 1] : (b + 1) * (a.p.T / a.p.B)) - first, a.p.T);
-    const int len = a.p.lengths[b], cap = a.p.width * a.c.page, p16 = a.c.page / 16;
+    const int len = kv4_length(a.p, b), cap = a.p.width * a.c.page, p16 = a.c.page / 16;
     const int* table = a.p.table + (size_t)b * a.p.width;
     const int rows = n * a.share;
 

@@ -81,3 +81,26 @@ def test_keys_of_any_finite_scale_give_finite_scores(D, group, length, new, scal
     args = (tuple(_cuda(x) for x in cache), _cuda(table), torch.tensor([length], dtype=torch.int32).cuda())
     for bounds in (dict(max_length=64), dict(max_tokens=new, max_length=5000)):
         _check(quant_hip.kv4_attention(_cuda(q), *args, **bounds), want, tol, bounds)
+
+
+@pytest.mark.parametrize("new", [1, 40, 150])
+def test_lengths_at_the_ends_of_32_bits(new):
+    """Far below zero: no key is seen and nothing is stored.  Far beyond the table: it ends with the table."""
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip
+    from oracle import kv4_oracle as o
+    rng = np.random.default_rng(new)
+    claimed = np.array([-2 ** 31, -2 ** 31 + new - 1, 2 ** 31 - 1, 2 ** 31 - 1 - new, 90], np.int64)
+    cache, table = _filled(o, [90] * 5, 1, 64, 64, 16, rng)
+    q = rng.standard_normal((5 * new, 1, 64)).astype(np.float16)
+    want, tol = o.attention(q, cache, table, claimed, None, 0.125, new > 64)
+    assert (want[:2 * new] == 0).all() and (want[2 * new:] != 0).any()
+    args = (tuple(_cuda(x) for x in cache), _cuda(table), torch.from_numpy(claimed.astype(np.int32)).cuda())
+    for bounds in (dict(), dict(max_tokens=new, max_length=5000)):
+        _check(quant_hip.kv4_attention(_cuda(q), *args, **bounds), want, tol, bounds)
+    k = torch.ones(5 * new, 1, 64, dtype=torch.float16, device="cuda")
+    before = [c.clone() for c in args[0]]
+    rope = torch.ones(8, 16, 2, device="cuda")
+    got = quant_hip.kv4_append(k[:4 * new], k[:4 * new], args[0], args[1][:4].contiguous(), args[2][:4].contiguous(), q=k[:4 * new], rope=rope)
+    assert bool((got == 0).all()) and all(torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(b.float())) for a, b in zip(before, args[0]))
+    assert not any(bool(t.any()) for t in quant_hip.kv4_read(args[0], args[1][:4].contiguous(), args[2][:4].contiguous(), 4 * new))
