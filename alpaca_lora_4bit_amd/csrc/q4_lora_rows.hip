@@ -8,7 +8,8 @@
 // rows.  Products are full 16-row tiles of v_mfma_f32_16x16x32_f16 either way; what a row's adapter did not make is not written.  HBM-bound: x and the used
 // adapters are read once, y once and written once; the second and later reads of an adapter by other tiles come from the caches.
 // x @ A^T * scaling goes to the matrix instructions as two fp16 numbers, the rounded one and what it left (ranks up to 16 have the room in one
-// instruction), so the update is rounded once, onto y.
+// instruction), times a power of two of the row's own that takes its largest between 2^14 and 2^15: sums far beyond fp16, or far below, lose nothing.  So the
+// update is rounded once, onto y.
 #include "q4_common.hpp"
 #include "q4_gptq.h"
 #include <algorithm>
@@ -134,6 +135,15 @@ __global__ __launch_bounds__(64 * kRowsWaves) void lora_rows_down_kernel(RowsArg
     }
 }
 
+// Maximum over P (2, 4 or 8) neighbouring lanes, all of them active.
+template <int P>
+__device__ __forceinline__ uint32_t max_of_pieces(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, false));                   // lanes 1, 0, 3, 2 of four
+    if constexpr (P > 2) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, false));     // lanes 2, 3, 0, 1
+    if constexpr (P > 4) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, false));    // lanes 7 .. 0 of eight
+    return x;
+}
+
 // ---- the update -------------------------------------------------------------------------------------
 // Workgroup = 256 columns, 64 a wavefront, of a tile of up to 16 * MT rows.  The sums become (rounded, rest) once, for all four; a wavefront's 64 rows of B and
 // its products pass through LDS too, so that every access to memory is of whole lines by neighbouring lanes.  y is requested first of all.
@@ -143,6 +153,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void lora_rows_up_kernel(RowsArgs 
     __shared__ half8_t sx[16 * MT][2 * P + 1];
     __shared__ half8_t sb[kRowsWaves][64][P + 1];
     __shared__ __attribute__((aligned(16))) float so[kRowsWaves][16][68];
+    __shared__ float back[16 * MT];                                        // what takes a row's products to their own size again
     const RowsProb& p = ra.p[blockIdx.z];
     const int lane = threadIdx.x & 63, r = lane & 15, kk = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -196,10 +207,22 @@ __global__ __launch_bounds__(64 * kRowsWaves) void lora_rows_up_kernel(RowsArgs 
             v += *reinterpret_cast<const float4_t*>(src + s * step);
             w += *reinterpret_cast<const float4_t*>(src + s * step + 4);
         }
+        v *= f;
+        w *= f;
+        uint32_t top = 0;                                                  // the row's largest magnitude; its P pieces lie in neighbouring lanes
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float z = e < 4 ? v[e & 3] : w[e & 3];
+            top = max(top, __builtin_bit_cast(uint32_t, z) & 0x7FFFFFFFu);
+        }
+        top = max_of_pieces<P>(top);
+        const int shift = top >= 0x7F800000u ? 0 : min(127 + 14 - (int)(top >> 23), 100);
+        const float grow = __builtin_bit_cast(float, (uint32_t)(127 + shift) << 23);
+        if (j == 0) back[row] = __builtin_bit_cast(float, (uint32_t)(127 - shift) << 23);
         half8_t hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float x = (e < 4 ? v[e & 3] : w[e & 3]) * f;
+            const float x = (e < 4 ? v[e & 3] : w[e & 3]) * grow;
             hi[e] = (half_t)x;
             lo[e] = __builtin_isinf((float)hi[e]) ? (half_t)0.f : (half_t)(x - (float)hi[e]);
         }
@@ -209,10 +232,13 @@ __global__ __launch_bounds__(64 * kRowsWaves) void lora_rows_up_kernel(RowsArgs 
     __syncthreads();
     if (!on) return;
     float4_t acc[MT][4];
+    float unit[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < MT; ++t) {
+        unit[t] = back[16 * t + r];                                        // of rows without an adapter: whatever, they are not written
 #pragma unroll
         for (int u = 0; u < 4; ++u) acc[t][u] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
     const int pieces = ra.R / 8;
     while (pending) {
         rows_next(idx, &pending, &mine);
@@ -259,7 +285,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void lora_rows_up_kernel(RowsArgs 
 #pragma unroll
     for (int t = 0; t < MT; ++t) {                                         // acc[t][u]: row 16*t + r, columns 16*u + 4*kk ..
 #pragma unroll
-        for (int u = 0; u < 4; ++u) *reinterpret_cast<float4_t*>(&so[wave][r][16 * u + 4 * kk]) = acc[t][u];
+        for (int u = 0; u < 4; ++u) *reinterpret_cast<float4_t*>(&so[wave][r][16 * u + 4 * kk]) = acc[t][u] * unit[t];
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
