@@ -294,18 +294,19 @@ def generate_batch(model, prompts, max_new_tokens, bank=None, adapters=None, eos
 
         left = max_new_tokens - 1
         done = advance(torch.stack(first))
-        graph = None
+        graph, warm = None, not use_graph
         while left and not done:
             if graph is not None:
                 graph.replay()
-            elif left == max_new_tokens - 1 and use_graph and left > 1:
+            elif not warm:
                 # one eager step on a side stream first: every lazy allocation and per-layer check happens there
                 side = torch.cuda.Stream()
                 side.wait_stream(torch.cuda.current_stream())
                 with torch.cuda.stream(side):
                     logits = step()
                 torch.cuda.current_stream().wait_stream(side)
-            elif use_graph:
+                warm = True
+            elif use_graph and left > 1:
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph):
                     logits = step()
