@@ -16,6 +16,7 @@ classes.  Two ways here, both leaving the host model's own attention / MLP code 
   adapter of rank r_q + r_v whose B matrix is block-structured (zero rows for k_proj).
 """
 import json
+import math
 import os
 import re
 import threading
@@ -628,13 +629,23 @@ def _read_adapter_state(lora_path):
     return torch.load(os.path.join(lora_path, "adapter_model.bin"), map_location="cpu", weights_only=True)
 
 
+def adapter_factor(cfg, path):
+    """What the update of the layer at `path` is multiplied by, from a saved adapter's configuration: lora_alpha / r, or lora_alpha / sqrt(r) with
+    `use_rslora`; `alpha_pattern` and `rank_pattern` give some layers an alpha and a rank of their own, each key a pattern for the end of a layer's path."""
+    def of(patterns, common):
+        return next((value for key, value in (patterns or {}).items() if re.match(rf'(.*\.)?({key})$', path)), common)
+    alpha, r = of(cfg.get('alpha_pattern'), cfg['lora_alpha']), of(cfg.get('rank_pattern'), cfg['r'])
+    return alpha / math.sqrt(r) if cfg.get('use_rslora') else alpha / r
+
+
 _ADAPTER_KEY = re.compile(r"^(?:base_model\.model\.)?(.*)\.(q_proj|k_proj|v_proj)\.lora_([AB])(?:\.[^.]+)?\.weight$")
 
 
 def inject_lora_layers(model, lora_path, device='cuda', dtype=torch.float16):
     """Loads the adapter saved under `lora_path` (adapter_config.json + adapter_model.safetensors / .bin) onto the
     attention projections.  Same call as the reference's (model_attn_mlp_patch.py:283-335: q_proj and v_proj adapters,
-    scaling = lora_alpha / r, a second call replaces the adapter of the first); k_proj adapters are accepted as well.
+    scaling = lora_alpha / r, a second call replaces the adapter of the first); k_proj adapters and other factors of the
+    configuration (`adapter_factor`) are accepted as well.
     On a block fused with `concatenate=True` the adapters become one block-structured adapter on `qkv_proj`; on a block
     grouped in place (or not fused at all) every projection named in the file becomes a LoRA layer of its own that
     shares the projection's packed tensors and keeps its place in the group.  Returns the injected layers."""
@@ -642,7 +653,6 @@ def inject_lora_layers(model, lora_path, device='cuda', dtype=torch.float16):
     print('Device: {}, dtype: {}'.format(device, dtype))
     with open(os.path.join(lora_path, 'adapter_config.json'), 'r') as fh:
         cfg = json.load(fh)
-    scaling = cfg['lora_alpha'] / cfg['r']
 
     per_block = {}                                           # attention module path -> {(proj, 'A'|'B'): tensor}
     for key, tensor in _read_adapter_state(lora_path).items():
@@ -650,7 +660,7 @@ def inject_lora_layers(model, lora_path, device='cuda', dtype=torch.float16):
         if m is not None:
             per_block.setdefault(m.group(1), {})[(m.group(2), m.group(3))] = tensor
 
-    def lora_layer(base, a, b):
+    def lora_layer(base, a, b, scaling):
         # lora_alpha = scaling * rank keeps the layer's own scaling (lora_alpha / r) at the saved adapter's value
         rank = a.shape[0]
         layer = Linear4bitLt('default', base.in_features, base.out_features, base.groupsize, False,
@@ -673,14 +683,17 @@ def inject_lora_layers(model, lora_path, device='cuda', dtype=torch.float16):
         fused = getattr(attn, 'qkv_proj', None)
         if isinstance(fused, Autograd4bitQuantLinear):       # concatenated block: one block-structured adapter
             rank = sum(parts[(n, 'A')].shape[0] for n in present)
+            factors = {n: adapter_factor(cfg, f'{path}.{n}') for n in present}
+            scaling = next((f for f in factors.values() if f), 1.0)    # the others' factors, where they differ, go into B
             a_cat = torch.cat([parts[(n, 'A')].to(device=device, dtype=dtype) for n in present], dim=0)
             b_blk = torch.zeros(fused.out_features, rank, device=device, dtype=dtype)
             col = 0
             for n in present:
-                b = parts[(n, 'B')].to(device=device, dtype=dtype)
+                b = parts[(n, 'B')]
+                b = (b if factors[n] == scaling else b.float() * (factors[n] / scaling)).to(device=device, dtype=dtype)
                 b_blk[projs[n]._start:projs[n]._stop, col:col + b.shape[1]] = b
                 col += b.shape[1]
-            layer = lora_layer(fused, a_cat, b_blk)
+            layer = lora_layer(fused, a_cat, b_blk, scaling)
             attn.qkv_proj = layer
             projs['q_proj']._group.layer = layer
             injected.append(layer)
@@ -689,7 +702,8 @@ def inject_lora_layers(model, lora_path, device='cuda', dtype=torch.float16):
             base = projs[n]
             if not isinstance(base, Autograd4bitQuantLinear) or base.is_v1_model:
                 raise ValueError(f'{path}.{n} is not a 4-bit (v2) layer')
-            layer = lora_layer(base, parts[(n, 'A')].to(device=device, dtype=dtype), parts[(n, 'B')].to(device=device, dtype=dtype))
+            layer = lora_layer(base, parts[(n, 'A')].to(device=device, dtype=dtype), parts[(n, 'B')].to(device=device, dtype=dtype),
+                               adapter_factor(cfg, f'{path}.{n}'))
             group = base.__dict__.get('_q4_group')
             setattr(attn, n, layer)
             if group is not None:

@@ -335,17 +335,18 @@ class AdapterBank:
         the list is adapter i of the index that `apply` takes."""
         import json
         import os
-        from .model_attn_mlp_patch import _read_adapter_state
+        from .model_attn_mlp_patch import _read_adapter_state, adapter_factor
         modules = dict(model.named_modules())
-        parts, scalings = {}, []                             # module -> {(adapter, 'lora_A' | 'lora_B'): tensor}
+        parts, names, factors = {}, {}, []                   # module -> {(adapter, 'A' | 'B'): tensor}, its path; by adapter: the factor of a path
         for number, source in enumerate(adapters):
             if isinstance(source, (str, os.PathLike)):
                 with open(os.path.join(source, "adapter_config.json")) as fh:
                     cfg = json.load(fh)
-                state, scaling = _read_adapter_state(source), cfg["lora_alpha"] / cfg["r"]
+                state = _read_adapter_state(source)
+                factors.append(lambda path, cfg=cfg: adapter_factor(cfg, path))
             else:
                 state, scaling = source
-            scalings.append(float(scaling))
+                factors.append(lambda path, scaling=scaling: scaling)
             for key, tensor in state.items():
                 path = key[len("base_model.model."):] if key.startswith("base_model.model.") else key
                 name, dot, part = path.partition(".lora_")
@@ -358,7 +359,8 @@ class AdapterBank:
                 if tensor.dim() != 2 or tensor.shape[1 if part[0] == "A" else 0] != want:
                     raise ValueError(f"adapter {number}: {key} is {tuple(tensor.shape)}, the layer has {layer.in_features} -> {layer.out_features}")
                 parts.setdefault(layer, {})[(number, part[0])] = tensor
-        self.count = len(scalings)
+                names[layer] = name
+        self.count = len(factors)
         self._layers = {}
         for layer, found in parts.items():
             rank = 0
@@ -378,7 +380,7 @@ class AdapterBank:
                     a[number, :tensor.shape[0]] = tensor
                 else:
                     b[number, :, :tensor.shape[1]] = tensor
-            has = [s if (n, "A") in found else 0.0 for n, s in enumerate(scalings)]
+            has = [float(factor(names[layer])) if (n, "A") in found else 0.0 for n, factor in enumerate(factors)]
             self._layers[layer] = (a, b, torch.tensor(has, dtype=torch.float32).to(device))
 
     def holds(self, *layers):
