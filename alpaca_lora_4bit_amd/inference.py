@@ -154,6 +154,12 @@ class _BatchModel:
         from .kv4_cache import rope_table
         cfg = model.config
         self.model, self.cache, self.bank = model, cache, bank
+        if bank is not None:
+            taken = {getattr(part, n, None) for block in model.model.layers for part, names in ((block.self_attn, "qkvo"), (block.mlp, ("gate", "up", "down")))
+                     for n in (f"{x}_proj" for x in names)}
+            for layer, name in bank.names.items():
+                if layer not in taken:
+                    raise ValueError(f"the bank has an adapter of {name or 'a layer'}, which a batch of requests does not add")
         self.heads, self.kv_heads, self.head_dim = _attention_shape(cfg)
         self.rope = rope_table(model.model.rotary_emb, positions, cache.device)
 

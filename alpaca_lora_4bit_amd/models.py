@@ -337,7 +337,7 @@ class AdapterBank:
         import os
         from .model_attn_mlp_patch import _read_adapter_state, adapter_factor
         modules = dict(model.named_modules())
-        parts, names, factors = {}, {}, []                   # module -> {(adapter, 'A' | 'B'): tensor}, its path; by adapter: the factor of a path
+        parts, factors, self.names = {}, [], {}              # module -> {(adapter, 'A' | 'B'): tensor}; by adapter: the factor of a path; module -> its path
         for number, source in enumerate(adapters):
             if isinstance(source, (str, os.PathLike)):
                 with open(os.path.join(source, "adapter_config.json")) as fh:
@@ -359,7 +359,7 @@ class AdapterBank:
                 if tensor.dim() != 2 or tensor.shape[1 if part[0] == "A" else 0] != want:
                     raise ValueError(f"adapter {number}: {key} is {tuple(tensor.shape)}, the layer has {layer.in_features} -> {layer.out_features}")
                 parts.setdefault(layer, {})[(number, part[0])] = tensor
-                names[layer] = name
+                self.names[layer] = name
         self.count = len(factors)
         self._layers = {}
         for layer, found in parts.items():
@@ -380,7 +380,7 @@ class AdapterBank:
                     a[number, :tensor.shape[0]] = tensor
                 else:
                     b[number, :, :tensor.shape[1]] = tensor
-            has = [float(factor(names[layer])) if (n, "A") in found else 0.0 for n, factor in enumerate(factors)]
+            has = [float(factor(self.names[layer])) if (n, "A") in found else 0.0 for n, factor in enumerate(factors)]
             self._layers[layer] = (a, b, torch.tensor(has, dtype=torch.float32).to(device))
 
     def holds(self, *layers):
