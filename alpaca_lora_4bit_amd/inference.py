@@ -146,6 +146,47 @@ def greedy_generate_graph(model, input_ids, max_new_tokens, eos_token_id=None):
     return generate_graph(model, input_ids, max_new_tokens, eos_token_id=eos_token_id)
 
 
+def _passed_by(module, cls):
+    """What would be left out if `module`, in whose place a batch runs its parts, were not called: a hook, or a forward that is not the one of
+    transformers' LLaMA class `cls`.  None where there is no such thing: this package's groups and its wrappers of a forward (autocast,
+    checkpointing, the fused MLP step) are known to change nothing here."""
+    from .gradient_checkpointing import _ForwardPatch
+    from .model_attn_mlp_patch import _FusedGroup, _MemberGroup, _mlp_decode_forward
+    for hooks in (module._forward_hooks, module._forward_pre_hooks, module._backward_hooks, module._backward_pre_hooks):
+        if any(not isinstance(getattr(h, "__self__", None), (_FusedGroup, _MemberGroup)) for h in hooks.values()):
+            return "a hook"
+    own = module.__dict__
+    forward = own.get("forward")
+    if "_q4_mlp_forward" in own and getattr(forward, "__func__", None) is _mlp_decode_forward:
+        forward = own["_q4_mlp_forward"]
+    elif "non_autocast_forward" in own and getattr(forward, "__wrapped__", None) is own["non_autocast_forward"]:
+        forward = own["non_autocast_forward"]
+    elif "old_forward_for_cp" in own and isinstance(getattr(forward, "__self__", None), _ForwardPatch):
+        forward = own["old_forward_for_cp"]
+    if forward is not None and getattr(forward, "__func__", None) is not type(module).forward:
+        return "a replaced forward"
+    stock = type(module).forward
+    if (stock.__module__, stock.__qualname__) != ("transformers.models.llama.modeling_llama", f"{cls}.forward"):
+        return "a forward that is not LLaMA's"
+    return None
+
+
+def _check_blocks(model, bank):
+    """Everything that a batch takes apart is as it knows it (ValueError otherwise)."""
+    if torch.nn.modules.module._has_any_global_hook():
+        raise ValueError("batches of requests do not call every module: a global module hook would miss some")
+    net = model.model
+    parts = [("the model", model, "LlamaForCausalLM"), ("model", net, "LlamaModel")]
+    for i, block in enumerate(net.layers):
+        parts += [(f"model.layers.{i}", block, "LlamaDecoderLayer"), (f"model.layers.{i}.self_attn", block.self_attn, "LlamaAttention")]
+        if bank is not None and bank.holds(*(getattr(block.mlp, n, None) for n in ("gate_proj", "up_proj", "down_proj"))):
+            parts.append((f"model.layers.{i}.mlp", block.mlp, "LlamaMLP"))
+    for name, module, cls in parts:
+        what = _passed_by(module, cls)
+        if what is not None:
+            raise ValueError(f"batches of requests take {name} apart, which has {what} that they would leave out")
+
+
 class _BatchModel:
     """A LLaMA's blocks over rows of many sequences: the modules of the loaded model do the products and norms, the keys and values go through
     the 4-bit paged cache and every row's own adapter is added to the products."""
@@ -154,6 +195,7 @@ class _BatchModel:
         from .kv4_cache import rope_table
         cfg = model.config
         self.model, self.cache, self.bank = model, cache, bank
+        _check_blocks(model, bank)
         if bank is not None:
             taken = {getattr(part, n, None) for block in model.model.layers for part, names in ((block.self_attn, "qkvo"), (block.mlp, ("gate", "up", "down")))
                      for n in (f"{x}_proj" for x in names)}
