@@ -765,14 +765,27 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
     return reinterpret_cast<uintptr_t>(a.data_ptr()) < last(b) && reinterpret_cast<uintptr_t>(b.data_ptr()) < last(a);
 }
 
-// The result's tensor: a new one, or the caller's, which may be `like` itself but not another piece of its memory.
-at::Tensor rows_out(const c10::optional<at::Tensor>& out, int64_t T, int64_t H, int64_t D, const at::Tensor& like, const char* what) {
+// The bytes of a contiguous tensor, and whether two such pieces have some in common.
+struct Bytes {
+    uintptr_t first, end;
+    explicit Bytes(const at::Tensor& t) : first(reinterpret_cast<uintptr_t>(t.data_ptr())), end(first + t.nbytes()) {}
+    bool meets(const Bytes& o) const { return first < o.end && o.first < end && first < end && o.first < o.end; }
+};
+
+// The result's tensor: a new one, or the caller's, which may be `like` itself but neither another piece of its memory nor of what the kernels read beside it.
+at::Tensor rows_out(const c10::optional<at::Tensor>& out, int64_t T, int64_t H, int64_t D, const at::Tensor& like, const Kv4Tensors& cache,
+                    std::initializer_list<const at::Tensor*> read, const char* what) {
     if (!out.has_value()) return at::empty({T, H, D}, like.options());
     TORCH_CHECK_VALUE(out->scalar_type() == at::kHalf && out->dim() == 3 && out->size(0) == T && out->size(1) == H && out->size(2) == D &&
                       out->is_contiguous() && out->device() == like.device() && reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0, what,
                       " must be a contiguous, 16-byte aligned float16 [", T, ", ", H, ", ", D, "] tensor on the cache's device");
     check_no_grad(*out, what);
     TORCH_CHECK_VALUE((out->data_ptr() == like.data_ptr() && like.is_contiguous()) || !overlap(*out, like), what, " overlaps the queries");
+    const Bytes mine(*out);
+    bool apart = !mine.meets(Bytes(std::get<0>(cache))) && !mine.meets(Bytes(std::get<1>(cache))) && !mine.meets(Bytes(std::get<2>(cache))) &&
+                 !mine.meets(Bytes(std::get<3>(cache)));
+    for (const at::Tensor* t : read) apart = apart && (!t || !mine.meets(Bytes(*t)));
+    TORCH_CHECK_VALUE(apart, what, " overlaps the cache or another tensor of the call");
     return *out;
 }
 
@@ -788,7 +801,6 @@ c10::optional<at::Tensor> kv4_append(const at::Tensor& k, const at::Tensor& v, c
     if (q.has_value()) {
         q3 = check_heads(*q, T, c.cache.D, c.device, false, "q");
         TORCH_CHECK_VALUE(!q_out.has_value() || (!overlap(*q_out, k) && !overlap(*q_out, v)), "q_out overlaps k or v");
-        o = rows_out(q_out, T, q->size(1), c.cache.D, *q, "q_out");
     } else {
         TORCH_CHECK_VALUE(!q_out.has_value(), "q_out needs q");
     }
@@ -803,7 +815,9 @@ c10::optional<at::Tensor> kv4_append(const at::Tensor& k, const at::Tensor& v, c
                           "rope must turn a multiple of 16 dimensions, at most the head's, at one position at least");
     }
     c10::optional<at::Tensor> result;
-    if (q.has_value()) result = o;
+    if (q.has_value())
+        result = o = rows_out(q_out, T, q->size(1), c.cache.D, *q, cache, {&table, &lengths, starts.has_value() ? &*starts : nullptr,
+                                                                           rope.has_value() ? &*rope : nullptr}, "q_out");
     if (T == 0) return result;
     Launch L(c.device);
     const int rc = q4_kv4_append_f16(&c.cache, &c.batch, k3.data_ptr(), k3.stride(0), k3.stride(1), v3.data_ptr(), v3.stride(0), v3.stride(1),
@@ -837,7 +851,7 @@ at::Tensor kv4_attention(const at::Tensor& q, const Kv4Tensors& cache, const at:
     TORCH_CHECK_VALUE(H >= 1 && H % c.cache.heads == 0, "q must have a multiple of the cache's ", c.cache.heads, " heads, got ", H);
     if (scale == 0.0) scale = 1.0 / std::sqrt((double)c.cache.D);
     TORCH_CHECK_VALUE(scale > 0.0 && scale < 1e30, "scale must be positive and finite");
-    const at::Tensor o = rows_out(out, T, H, c.cache.D, q, "out");
+    const at::Tensor o = rows_out(out, T, H, c.cache.D, q, cache, {&table, &lengths, starts.has_value() ? &*starts : nullptr}, "out");
     if (T == 0) return o;
     const int64_t all = (int64_t)c.batch.width * c.cache.page, most = starts.has_value() ? T : T / c.batch.B;
     TORCH_CHECK_VALUE((!max_tokens.has_value() || *max_tokens >= 1) && (!max_length.has_value() || *max_length >= 1),
@@ -865,6 +879,8 @@ void lora_rows(const at::Tensor& x, const at::Tensor& index, const std::vector<R
     TORCH_CHECK_VALUE(per >= 1 && index.scalar_type() == at::kInt && index.dim() == 1 && index.is_contiguous() && index.device() == x.device() &&
                       index.size(0) == (M == 0 ? 0 : (M - 1) / per + 1), "index must be a contiguous int32 tensor on x's device, one entry for each ", per, " rows");
     q4_lora_rows_t probs[4];
+    c10::SmallVector<Bytes, 4> written;
+    c10::SmallVector<Bytes, 14> read = {Bytes(x), Bytes(index)};
     int64_t n = 0, R = 0;
     for (size_t i = 0; i < count; ++i) {
         const at::Tensor &a = std::get<0>(specs[i]), &b = std::get<1>(specs[i]), &s = std::get<2>(specs[i]), &y = std::get<3>(specs[i]);
@@ -879,16 +895,20 @@ void lora_rows(const at::Tensor& x, const at::Tensor& index, const std::vector<R
         TORCH_CHECK_VALUE(y.scalar_type() == at::kHalf && y.dim() == 2 && y.size(0) == M && y.size(1) == b.size(1) && y.is_contiguous() &&
                           y.device() == x.device(), "y must be a contiguous float16 [M, N] tensor on x's device");
         check_no_grad(s, "scaling");
-        TORCH_CHECK_VALUE(!overlap(y, x) && !overlap(y, a) && !overlap(y, b), "y overlaps another tensor of the call");
-        for (size_t j = 0; j < i; ++j)
-            TORCH_CHECK_VALUE(!overlap(y, std::get<3>(specs[j])) && !overlap(y, std::get<0>(specs[j])) && !overlap(y, std::get<1>(specs[j])) &&
-                              !overlap(a, std::get<3>(specs[j])) && !overlap(b, std::get<3>(specs[j])), "y overlaps another tensor of the call");
+        written.emplace_back(y);
+        for (const at::Tensor* t : {&a, &b, &s}) read.emplace_back(*t);
         for (const at::Tensor* t : {&a, &b, &y}) {
             check_no_grad(*t, "a tensor of lora_rows");
             TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "the tensors of lora_rows must be 16-byte aligned");
         }
         TORCH_CHECK_VALUE(y.size(1) >= 64 && y.size(1) % 64 == 0 && y.size(1) <= (1 << 23), "N must be a multiple of 64");
         probs[i] = {a.data_ptr(), b.data_ptr(), s.data_ptr<float>(), y.data_ptr(), (int)y.size(1)};
+    }
+    for (size_t i = 0; i < count; ++i) {
+        bool apart = true;
+        for (const Bytes& r : read) apart = apart && !written[i].meets(r);
+        for (size_t j = 0; j < i; ++j) apart = apart && !written[i].meets(written[j]);
+        TORCH_CHECK_VALUE(apart, "y overlaps another tensor of the call");
     }
     TORCH_CHECK_VALUE(R >= 8 && R <= 64 && R % 8 == 0, "the rank must be a multiple of 8 in [8, 64], got ", R);
     TORCH_CHECK_VALUE(K >= 32 && K % 32 == 0 && K <= (1 << 20) && M <= (1 << 24), "K must be a multiple of 32 up to 2^20, and x have up to 2^24 rows");
