@@ -694,8 +694,9 @@ void reset_workspaces() {
 // Workspaces come from the caching allocator call by call, not from this stream's buffers: a captured graph then owns its own, and two graphs
 // that were captured on one stream may be replayed side by side.
 
-// Inference only: a result would silently miss its gradient.
+// Inference only: a result would silently miss its gradient, or its tangent in forward mode.
 void check_no_grad(const at::Tensor& t, const char* what) {
+    TORCH_CHECK_VALUE(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()), what, " has a tangent: this operator has no forward mode");
     TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), what, " requires grad: this operator has no backward pass");
 }
 
@@ -715,6 +716,8 @@ Kv4 check_kv4(const Kv4Tensors& c, const at::Tensor& table, const at::Tensor& le
                       "page, D/8] and v_codes int32 [pages, heads, page/4, D/8, 4]");
     TORCH_CHECK_VALUE(ks.scalar_type() == at::kHalf && ks.dim() == 4 && vs.scalar_type() == at::kHalf && vs.sizes() == ks.sizes(),
                       "k_scales and v_scales must be float16 [pages, heads, D/group, page]");
+    check_no_grad(ks, "k_scales");
+    check_no_grad(vs, "v_scales");
     const int64_t P = kc.size(0), H = kc.size(1), page = kc.size(2), D = kc.size(3) * 8, NG = ks.size(2);
     TORCH_CHECK_VALUE(P >= 1 && page >= 16 && page <= 1024 && page % 16 == 0, "pages must hold a multiple of 16 tokens, up to 1024; got ", page);
     TORCH_CHECK_VALUE(D == 64 || D == 128, "heads must be 64 or 128 wide, got ", D);
@@ -809,6 +812,7 @@ c10::optional<at::Tensor> kv4_append(const at::Tensor& k, const at::Tensor& v, c
         TORCH_CHECK_VALUE(rope->scalar_type() == at::kFloat && rope->dim() == 3 && rope->size(2) == 2 && rope->is_contiguous() && rope->device() == c.device &&
                           reinterpret_cast<uintptr_t>(rope->data_ptr()) % 16 == 0,
                           "rope must be a contiguous float32 [positions, rotated/2, 2] tensor on the cache's device");
+        check_no_grad(*rope, "rope");
         rows = rope->size(0);
         rot = 2 * rope->size(1);
         TORCH_CHECK_VALUE(rows >= 1 && rows < (1ll << 31) && rot >= 16 && rot <= c.cache.D && rot % 16 == 0,
