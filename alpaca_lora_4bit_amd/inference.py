@@ -20,6 +20,7 @@ otherwise the reference's sampling settings) runs eagerly between two replays.
 (kv4_cache.py) and their adapters beside each other (models.AdapterBank); see `generate_batch`.
 """
 import argparse
+import contextlib
 import json
 import time
 
@@ -249,6 +250,15 @@ def _attention_shape(cfg):
     return heads, getattr(cfg, "num_key_value_heads", None) or heads, getattr(cfg, "head_dim", None) or cfg.hidden_size // heads
 
 
+_capture_streams = {}                                        # by device: torch's own is one for all, on the device that captured first
+
+
+def _capture_stream(dev):
+    if dev.index not in _capture_streams:
+        _capture_streams[dev.index] = torch.cuda.Stream(dev)
+    return _capture_streams[dev.index]
+
+
 def generate_batch(model, prompts, max_new_tokens, bank=None, adapters=None, eos_token_id=None, sampling=None, use_graph=True,
                    page=64, group=32, prefill_rows=8192):
     """Continues many prompts together.  `prompts`: 1-D id tensors, of any lengths; `adapters`: for each of them the number of its adapter in
@@ -275,7 +285,7 @@ def generate_batch(model, prompts, max_new_tokens, bank=None, adapters=None, eos
     pages = sum(-(-t // page) for t in totals)
     pick = _token_picker(sampling)
     ints = dict(dtype=torch.int32)
-    with torch.no_grad():
+    with torch.no_grad(), torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext():
         cache = PagedKv4Cache(len(model.model.layers), kv_heads, head_dim, pages, page, group, dev)
         run = _BatchModel(model, cache, bank, longest)
         handles = [cache.open(t) for t in totals]
@@ -348,15 +358,15 @@ def generate_batch(model, prompts, max_new_tokens, bank=None, adapters=None, eos
                 graph.replay()
             elif not warm:
                 # one eager step on a side stream first: every lazy allocation and per-layer check happens there
-                side = torch.cuda.Stream()
-                side.wait_stream(torch.cuda.current_stream())
+                side = torch.cuda.Stream(dev)
+                side.wait_stream(torch.cuda.current_stream(dev))
                 with torch.cuda.stream(side):
                     logits = step()
-                torch.cuda.current_stream().wait_stream(side)
+                torch.cuda.current_stream(dev).wait_stream(side)
                 warm = True
             elif use_graph and left > 1:
                 graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(graph):
+                with torch.cuda.graph(graph, stream=_capture_stream(dev)):
                     logits = step()
                 graph.replay()
             else:

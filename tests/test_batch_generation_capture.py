@@ -25,6 +25,9 @@ def events(monkeypatch):
     monkeypatch.setattr(quant_hip, "kv4_append", counted)
 
     class Stream:
+        def __init__(self, device=None):
+            assert device is not None and device.type == "cpu"           # where the prompts are
+
         def wait_stream(self, other):
             pass
 
@@ -33,11 +36,13 @@ def events(monkeypatch):
             seen.append(("replay", -1))
 
     @contextlib.contextmanager
-    def graph(g):
+    def graph(g, stream):
+        assert isinstance(stream, Stream)
         inside.append(g)
         yield
         inside.pop()
-    for name, value in (("Stream", lambda *a: Stream()), ("current_stream", lambda *a: Stream()), ("stream", lambda s: contextlib.nullcontext()), ("CUDAGraph", Graph), ("graph", graph)):
+    monkeypatch.setattr(inference, "_capture_streams", {})
+    for name, value in (("Stream", Stream), ("current_stream", Stream), ("stream", lambda s: contextlib.nullcontext()), ("CUDAGraph", Graph), ("graph", graph)):
         monkeypatch.setattr(torch.cuda, name, value)
     return seen
 
