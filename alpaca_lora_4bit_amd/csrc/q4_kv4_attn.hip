@@ -4,7 +4,8 @@
 //
 // One pass over the keys with the running maximum m and sum l of the softmax in fp32.  Codes go to the matrix instructions as the exact
 // fp16 values that they stand for; the keys' scales multiply the fp32 scores, the values' scales the probabilities, whose rounding to
-// fp16 is the only one before the output's (prompts round more, see there).
+// fp16 is the only one before the output's (prompts round more, see there).  What it costs beside the output's own rounding: nothing that shows for values' scales
+// of 0.3 down to 1e-5 over 100000 keys (root mean square 2.1e-4 to 8.8e-4 with it and without).
 #include "q4_kv4.hpp"
 #include <algorithm>
 #include <type_traits>
@@ -325,18 +326,19 @@ __global__ __launch_bounds__(256, 3) void kv4_attn_rows_kernel(Kv4Attn a) {
 //   values' piece (kb, p, db, lane): dimension 32*db + r of keys 32*kb + 16*p + 4*h + (0..3) and + 8, the keys of the scores in that lane's registers 8*p .. + 7
 // The maximum that weights refer to is raised only when a score lies 2^kSlack above it: weights then stay below 2^15.
 //
-// Rows that see up to kFewKeys keys get the keys' codes as they are, and each group's fp32 sums times its keys' scales; for rows that see more, code * scale is
+// Blocks of rows whose last one sees up to kFewKeys keys get the keys' codes as they are, and each group's fp32 sums times its keys' scales; in blocks that see more, code * scale is
 // rounded once like the values.  Root mean square error of a whole output against float64, relative: 2.6e-4 so, 3.1e-4 with all rounded for the prompt of 2048 tokens, 2.6e-4 and 3.4e-4
-// for one of 128 (2.1e-4 are the output's own rounding), but 2.4e-4 rounded where 4096 keys average it; exact keys cost 5, 15 and 40 per cent at 1, 2 and 4 groups.
+// for one of 128, 2.3e-4 for parts of prompts that see thousands (2.1e-4 are the output's own rounding); exact keys cost 5, 15 and 40 per cent at 1, 2 and 4 groups.
 //
 // What bounds it: a wavefront starts an operation in about eight cycles, and two of them share a SIMD, whose vector operations (230 a tile and wavefront) and matrix
-// operations (32 of 32 cycles) take 1900 of the 3250 to 4400 cycles that a tile of both lasts at 2.1 GHz.  The whole prompt of 2048 tokens, 32 heads of 128: 64 us, of which the
-// last block's 32 tiles are 55; parts of four prompts (509, 434, 360, 286 tokens at 8191, 5062, 1933, 6995; 8 key heads of 4): 195 us, 128 tiles one after the other.
+// operations (32 of 32 cycles) take 1900 of the 3700 cycles that a tile of both lasts at 2.1 GHz.  The whole prompt of 2048 tokens, 32 heads of 128: 59 us, of which the
+// last block's 32 tiles are 55; parts of four prompts (509, 434, 360, 286 tokens at 8191, 5062, 1933, 6995; 8 key heads of 4): 196 us, 128 tiles one after the other.
 // Eight wavefronts on 256 rows, half turning keys, half values: 69 and 216 us, for all are at the same step; splitting the keys of whole prompts costs the join more
 // than the balance gives (parts: 271 us in two shares).
 //
 // Values beyond fp16 (a scale above 10912, whose sixfold passes it; append writes none) would be infinite in LDS, and nothing times infinity is no number
-// for the rows that do not see them.  The staging finds such a scale, and the rows are gone through a second time with an eighth of every value, which holds all of them.
+// for the rows that do not see them.  The staging finds such a scale, and the rows are gone through a second time with an eighth of every value, which holds all of them.  (Once per block of rows that has such a
+// value; the test for it replaces one for infinities, operation for operation; that there may be a second pass costs the others under 1 per cent.)
 // Rounded keys are eighths always (a rotation takes pairs of large numbers beyond fp16; the conversion from codes multiplies by a power of two for nothing), and the softmax
 // scale is eightfold; keys below 2^-11 lose up to three bits by it.
 constexpr uint32_t kMostValueScale = 0x7154u;          // 10912 in fp16

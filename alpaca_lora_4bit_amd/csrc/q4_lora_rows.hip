@@ -4,7 +4,7 @@
 //
 // for up to four layers that share x and the index (q | k | v).  The adapters of a layer are one bank, A [n, R, K] and B [n, N, R].
 // Two launches: `down` leaves x @ A^T in fp32, as one sum or as sums over a few shares of K, `up` adds those in a fixed order and makes the update.  A
-// tile of 1 to 64 rows, in any order, is gone through adapter by adapter: the rows of one prompt have one, a tile of a decode batch as many as
+// tile of 1 to 32 rows, in any order, is gone through adapter by adapter: the rows of one prompt have one, a tile of a decode batch as many as
 // rows.  Products are full 16-row tiles of v_mfma_f32_16x16x32_f16 either way; what a row's adapter did not make is not written.  HBM-bound: x and the used
 // adapters are read once, y once and written once; the second and later reads of an adapter by other tiles come from the caches.
 // x @ A^T * scaling goes to the matrix instructions as two fp16 numbers, the rounded one and what it left (ranks up to 16 have the room in one

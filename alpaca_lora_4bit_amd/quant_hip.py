@@ -1059,8 +1059,9 @@ def kv4_attention(q, cache, page_table, lengths, scale=None, starts=None, max_to
     """fp16 [rows, q_heads, D]: attention of every row over its sequence's keys at or before its own position, softmax(scale * q . k) v
     (scale None: 1/sqrt(D)), into `out` if given, which may be a contiguous q itself.  A row that sees no key comes out as zero; rows of no sequence are
     not written (a new result's are undefined).  `max_tokens`, the rows of the longest
-    run of new tokens, and `max_length`, the tokens of the longest sequence, size the launch (None: what the shapes allow); the result does not
-    depend on them being right."""
+    run of new tokens, and `max_length`, the tokens of the longest sequence, size the launch (None: what the shapes allow).  They need not be right, but they
+    choose the kernel, and with it speed and roundings: max_tokens * q_heads / heads above 64 is the prompts', which rounds values and, in blocks of rows that see more
+    than 1024, keys to fp16 on the way.  Decode steps with `starts` should pass max_tokens=1."""
     if scale is None:
         scale = 0.0
     else:

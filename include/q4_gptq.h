@@ -405,8 +405,9 @@ Q4_API int q4_kv4_read_f16(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *ba
 
 /* out fp16 [T, q_heads, D]: attention of each row over its sequence's keys at or before its own position, softmax(scale * q . k) v with
  * q fp16 (strides as above, multiples of 8), q head h on key head h / (q_heads / heads).  A row that sees no key comes out as zero; keys without a
- * place are not seen.  scale > 0; B * heads <= 2^22.  out may be q if that is contiguous.  `max_tokens` (rows of the longest sequence) and `max_length` (its tokens) size the launch; the result does not depend on
- * their being right.  `workspace`: the bytes that the query gives for the same arguments (0: may be NULL), 256-byte aligned, contents irrelevant. */
+ * place are not seen.  0 < scale < 1e37; B * heads <= 2^22.  out may be q if that is contiguous.  `max_tokens` (rows of the longest sequence) and `max_length` (its tokens) size the launch.  They need
+ * not be right, but choose the kernel, and with it speed and roundings: above 64 = max_tokens * q_heads / heads values and, in blocks of rows that see more than 1024, keys are
+ * rounded to fp16 on the way.  A scale of the cache that is no number makes a row that sees it none, and no other row.  `workspace`: the bytes that the query gives for the same arguments (0: may be NULL), 256-byte aligned, contents irrelevant. */
 Q4_API size_t q4_kv4_attention_workspace_bytes(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, int q_heads, int max_tokens, int max_length);
 Q4_API int q4_kv4_attention_f16(const q4_kv4_cache_t *cache, const q4_kv4_batch_t *batch, const void *q, long long q_t, long long q_h, int q_heads,
                          float scale, void *out, int max_tokens, int max_length, void *workspace, size_t workspace_bytes, void *stream);
