@@ -117,7 +117,8 @@ def attention(q, cache, table, lengths, starts, scale, rounded=False):
     Terms of tol: half a step of the output, 2^-11 |o| (2^-25 where it is subnormal); half a step of every weight, 2^-11 sum p |v|, or 2^-25 * 6 in units of
     2^10 for subnormal ones (fewer where scales above 32 raise the maximum); twice (numerator and denominator) the relative error of a weight, exp of a score that is off by (D + 8) float32 half steps of
     sum |q k| and whose product with scale and difference to the maximum (at most 2 max |s|) round, and two steps of the exponential; the sums over L keys, of at most
-    L / 32 + 64 additions one after the other.  `rounded`: a score is off by 2^-11 sum |q k| more (2^-25 sum |q| for subnormal keys), the values by 2^-11 sum p |v|
+    L / 32 + 64 additions one after the other.  `rounded`: a score is off by 2^-11 sum |q k| more (2^-25 sum |q| for subnormal keys, 2^-22 where
+    eighths of them are rounded: blocks of up to 128 rows whose last one sees more than 1024 keys), the values by 2^-11 sum p |v|
     and 2^-25."""
     pages, heads, page = cache[0].shape[:3]
     T, Hq, D = q.shape
@@ -148,7 +149,7 @@ def attention(q, cache, table, lengths, starts, scale, rounded=False):
                     eps = mag * (D + 8) * u + 4 * np.abs(s).max() * u + 4 * u
                     more, unit = 0.0, 6 * big
                     if rounded:
-                        eps += mag * 2.0 ** -11 + scale * np.abs(x).sum() * 2.0 ** -25
+                        eps += mag * 2.0 ** -11 + scale * np.abs(x).sum() * 2.0 ** (-22 if len(seen) > 1024 - 128 else -25)
                         more, unit = 2.0 ** -11 * pv + 2.0 ** -25, max(unit, np.abs(v).max())
                     L = len(seen)
                     out[t, qh] = o

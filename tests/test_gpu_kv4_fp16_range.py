@@ -104,3 +104,18 @@ def test_lengths_at_the_ends_of_32_bits(new):
     got = quant_hip.kv4_append(k[:4 * new], k[:4 * new], args[0], args[1][:4].contiguous(), args[2][:4].contiguous(), q=k[:4 * new], rope=rope)
     assert bool((got == 0).all()) and all(torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(b.float())) for a, b in zip(before, args[0]))
     assert not any(bool(t.any()) for t in quant_hip.kv4_read(args[0], args[1][:4].contiguous(), args[2][:4].contiguous(), 4 * new))
+
+
+def test_keys_below_the_normal_numbers_in_long_prompts():
+    """Keys of some 1e-5 and queries that make scores of order one of them: rounded as eighths, a half step of 2^-22 each."""
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip
+    from oracle import kv4_oracle as o
+    rng = np.random.default_rng(5)
+    length, new, D = 1200, 100, 64
+    cache, table = _filled(o, [length], 1, D, 64, 48, rng)
+    cache[2][:] = np.where(np.isnan(cache[2]), cache[2], np.float16(1e-5))
+    q = (rng.standard_normal((new, 1, D)) * 2000).astype(np.float16)
+    want, tol = o.attention(q, cache, table, np.array([length]), None, 1 / math.sqrt(D), True)
+    got = quant_hip.kv4_attention(_cuda(q), tuple(_cuda(x) for x in cache), _cuda(table), torch.tensor([length], dtype=torch.int32).cuda())
+    _check(got, want, tol)
