@@ -7,6 +7,7 @@ Sub-modules keep the reference's names so its callers read unchanged:
     models               Linear4bitLt, GPTQLoraModel
     monkeypatch.peft_tuners_lora_monkey_patch   replace_peft_model_with_int4_lora_model
     arg_parser, Finetune4bConfig, train_data, gradient_checkpointing   what the finetune script imports
+    preference           log-probabilities of answers and the loss of pairs of them (no counterpart in the reference)
     kv4_cache            the 4-bit paged key/value cache of many requests (no counterpart in the reference)
     finetune, inference  the reference's two top-level scripts as runnable modules (python -m ...)
 
@@ -23,7 +24,7 @@ __version__ = "0.1.0"
 
 _ALIASED = ("autograd_4bit", "matmul_utils_4bit", "quant_hip", "models", "amp_wrapper", "model_attn_mlp_patch",
             "loaders", "arg_parser", "Finetune4bConfig", "train_data", "gradient_checkpointing", "monkeypatch",
-            "monkeypatch.peft_tuners_lora_monkey_patch", "kv4_cache")
+            "monkeypatch.peft_tuners_lora_monkey_patch", "kv4_cache", "preference")
 
 
 def install_as_alpaca_lora_4bit(name: str = "alpaca_lora_4bit") -> None:

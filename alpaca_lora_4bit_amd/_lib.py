@@ -6,7 +6,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libq4gptq.so")
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 _lib = None
 
@@ -126,6 +126,22 @@ SIGNATURES["q4_kv4_attention_workspace_bytes"] = (_sz, _kv4 + [_i, _i, _i])
 SIGNATURES["q4_kv4_attention_f16"] = (_i, _kv4 + [_vp, _ll, _ll, _i, _f, _vp, _i, _i, _vp, _sz, _vp])
 SIGNATURES["q4_lora_rows_workspace_bytes"] = (_sz, [_i, _i, _i, _i])
 SIGNATURES["q4_lora_rows_f16"] = (_i, [ctypes.POINTER(LoraRows), _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp])
+
+
+class Act8(ctypes.Structure):
+    """q4_act8_t of include/q4_gptq.h."""
+    _fields_ = [("codes", _vp), ("scales", _vp)]
+
+
+_act8 = ctypes.POINTER(Act8)
+SIGNATURES["q4_act8_pack"] = (_i, [_vp, _i, _vp, _vp, _ll, _vp])
+SIGNATURES["q4_act8_unpack"] = (_i, [_vp, _vp, _vp, _i, _ll, _vp])
+SIGNATURES["q4_silu_mul_act8"] = (_i, [_vp, _vp, _i, _vp, _act8, _act8, _ll, _vp])
+SIGNATURES["q4_silu_mul_act8_bwd"] = (_i, [_vp, _i, _act8, _act8, _vp, _vp, _ll, _vp])
+SIGNATURES["q4_token_logps"] = (_i, [_vp, _i, _ll, _ll, _i, _i, _i, _vp, _vp, _vp, _vp])
+SIGNATURES["q4_token_logps_bwd"] = (_i, [_vp, _i, _ll, _ll, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp])
+SIGNATURES["q4_preference_loss_workspace_bytes"] = (_sz, [_i, _i])
+SIGNATURES["q4_preference_loss"] = (_i, [_vp, _i, _ll, _ll, _i, _i, _i, _vp, _vp, ctypes.c_double, ctypes.c_double, _vp, _vp, _vp, _vp, _vp, _sz, _vp])
 
 
 class Q4Error(RuntimeError):

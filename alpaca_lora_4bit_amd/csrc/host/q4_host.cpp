@@ -28,6 +28,7 @@ py::object g_error_class;      // alpaca_lora_4bit_amd._lib.Q4Error, set by Pyth
 
 [[noreturn]] void raise_q4(int code, const char* what) {
     const std::string msg = std::string(what) + ": " + q4_error_string(code) + " (code " + std::to_string(code) + ")";
+    if (!PyGILState_Check()) throw std::runtime_error(msg);        // a backward pass, on a thread of autograd's
     if (g_error_class && !g_error_class.is_none()) {
         PyErr_SetString(g_error_class.ptr(), msg.c_str());
         throw py::error_already_set();
@@ -927,6 +928,219 @@ void lora_rows(const at::Tensor& x, const at::Tensor& index, const std::vector<R
     if (rc != Q4_OK) raise_q4(rc, "q4_lora_rows_f16");
 }
 
+// ---- training on pairs of answers, and what a step keeps for its backward pass -------------------------------------------------
+// Tensors come from the caching allocator call by call, workspaces too.  The gradients are the Python layer's autograd functions'.
+
+int type_of(const at::Tensor& t, bool wide, const char* what) {
+    const auto s = t.scalar_type();
+    TORCH_CHECK_VALUE(s == at::kHalf || s == at::kBFloat16 || (wide && s == at::kFloat), what, wide ? " must be float16, bfloat16 or float32" : " must be float16 or bfloat16");
+    return s == at::kHalf ? Q4_TYPE_F16 : s == at::kBFloat16 ? Q4_TYPE_BF16 : Q4_TYPE_F32;
+}
+// The tensor itself or a copy of it that lies in one piece from a 16-byte boundary on.
+at::Tensor in_one_piece(const at::Tensor& t) {
+    if (t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
+    return at::empty(t.sizes(), t.options()).copy_(t);
+}
+void check_count(const at::Tensor& t, const char* what) {
+    TORCH_CHECK_VALUE(t.is_cuda(), what, " must be on the GPU");
+    TORCH_CHECK_VALUE(t.numel() < (1ll << 35) - 2048, what, " has too many values");
+    check_no_grad(t, what);
+}
+at::Tensor new_codes(const at::Tensor& like) { return at::empty(like.sizes(), like.options().dtype(at::kChar)); }
+at::Tensor new_scales(const at::Tensor& like) { return at::empty({(like.numel() + 31) / 32}, like.options().dtype(at::kBFloat16)); }
+// codes and scales of the same call, as the kernels take them
+void check_act8(const at::Tensor& codes, const at::Tensor& scales) {
+    check_count(codes, "codes");
+    check_no_grad(scales, "scales");
+    TORCH_CHECK_VALUE(codes.scalar_type() == at::kChar && codes.is_contiguous() && reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0,
+                      "codes must be a contiguous, 16-byte aligned int8 tensor");
+    TORCH_CHECK_VALUE(scales.scalar_type() == at::kBFloat16 && scales.dim() == 1 && scales.size(0) == (codes.numel() + 31) / 32 && scales.is_contiguous() &&
+                      scales.device() == codes.device() && reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
+                      "scales must be a contiguous, 16-byte aligned bfloat16 tensor on the codes' device, one for each 32 of them");
+}
+
+std::pair<at::Tensor, at::Tensor> act8_pack(const at::Tensor& x) {
+    check_count(x, "x");
+    const int type = type_of(x, true, "x");
+    const at::Tensor x1 = in_one_piece(x);
+    at::Tensor codes = new_codes(x), scales = new_scales(x);
+    if (x.numel() == 0) return {codes, scales};
+    Launch L(x.device());
+    const int rc = q4_act8_pack(x1.data_ptr(), type, codes.data_ptr(), scales.data_ptr(), x1.numel(), L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_act8_pack");
+    return {codes, scales};
+}
+
+at::Tensor act8_unpack(const at::Tensor& codes, const at::Tensor& scales, at::ScalarType dtype) {
+    check_act8(codes, scales);
+    at::Tensor x = at::empty(codes.sizes(), codes.options().dtype(dtype));
+    const int type = type_of(x, true, "dtype");
+    if (x.numel() == 0) return x;
+    Launch L(codes.device());
+    const int rc = q4_act8_unpack(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), type, x.numel(), L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_act8_unpack");
+    return x;
+}
+
+// (gate's codes, gate's scales, up's codes, up's scales)
+using Kept = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+std::pair<at::Tensor, Kept> silu_mul_act8(const at::Tensor& gate, const at::Tensor& up) {
+    check_count(gate, "gate");
+    check_count(up, "up");
+    const int type = type_of(gate, false, "gate");
+    TORCH_CHECK_VALUE(up.scalar_type() == gate.scalar_type() && up.sizes() == gate.sizes() && up.device() == gate.device(), "up must be like gate");
+    const at::Tensor g = in_one_piece(gate), u = in_one_piece(up);
+    at::Tensor out = at::empty(gate.sizes(), gate.options());
+    Kept kept{new_codes(gate), new_scales(gate), new_codes(gate), new_scales(gate)};
+    if (gate.numel() == 0) return {out, kept};
+    const q4_act8_t kg{std::get<0>(kept).data_ptr(), std::get<1>(kept).data_ptr()}, ku{std::get<2>(kept).data_ptr(), std::get<3>(kept).data_ptr()};
+    Launch L(gate.device());
+    const int rc = q4_silu_mul_act8(g.data_ptr(), u.data_ptr(), type, out.data_ptr(), &kg, &ku, gate.numel(), L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_silu_mul_act8");
+    return {out, kept};
+}
+
+std::pair<at::Tensor, at::Tensor> silu_mul_act8_bwd(const at::Tensor& dout, const Kept& kept) {
+    check_count(dout, "dout");
+    const int type = type_of(dout, false, "dout");
+    check_act8(std::get<0>(kept), std::get<1>(kept));
+    check_act8(std::get<2>(kept), std::get<3>(kept));
+    TORCH_CHECK_VALUE(std::get<0>(kept).sizes() == dout.sizes() && std::get<2>(kept).sizes() == dout.sizes() && std::get<0>(kept).device() == dout.device() &&
+                      std::get<2>(kept).device() == dout.device(), "dout must have the shape and device of what was kept");
+    const at::Tensor d = in_one_piece(dout);
+    at::Tensor dgate = at::empty(dout.sizes(), dout.options()), dup = at::empty(dout.sizes(), dout.options());
+    if (dout.numel() == 0) return {dgate, dup};
+    const q4_act8_t kg{std::get<0>(kept).data_ptr(), std::get<1>(kept).data_ptr()}, ku{std::get<2>(kept).data_ptr(), std::get<3>(kept).data_ptr()};
+    Launch L(dout.device());
+    const int rc = q4_silu_mul_act8_bwd(d.data_ptr(), type, &kg, &ku, dgate.data_ptr(), dup.data_ptr(), dout.numel(), L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_silu_mul_act8_bwd");
+    return {dgate, dup};
+}
+
+// Logits [..., V] as [B, S, V] with their strides, and the labels beside them.
+struct Answers {
+    at::Tensor logits, labels;
+    int64_t B, S, V;
+    int type;
+    const long long* label_ptr() const { return reinterpret_cast<const long long*>(labels.data_ptr<int64_t>()); }
+};
+Answers check_answers(const at::Tensor& logits, const at::Tensor& labels) {
+    TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() >= 1, "logits must be a [..., V] tensor on the GPU");
+    check_no_grad(logits, "logits");
+    Answers a;
+    a.type = type_of(logits, true, "logits");
+    a.V = logits.size(-1);
+    TORCH_CHECK_VALUE(labels.scalar_type() == at::kLong && labels.sizes() == logits.sizes().slice(0, logits.dim() - 1) && labels.device() == logits.device(),
+                      "labels must be an int64 tensor of logits' shape without its last dimension, on its device");
+    TORCH_CHECK_VALUE(a.V >= 1 && a.V < (1 << 30) && labels.numel() < (1ll << 31), "logits must have 1 to 2^30 - 1 words and fewer than 2^31 rows");
+    a.labels = labels.contiguous();
+    at::Tensor x = logits;
+    if (x.dim() < 3) x = x.unsqueeze(0);
+    if (x.dim() < 3) x = x.unsqueeze(0);
+    if (x.dim() > 3) x = x.reshape({-1, x.size(-2), a.V});
+    if (x.stride(2) != 1 && a.V > 1) x = x.contiguous();
+    a.logits = x;
+    a.B = x.size(0);
+    a.S = x.size(1);
+    return a;
+}
+
+std::pair<at::Tensor, at::Tensor> token_logps(const at::Tensor& logits, const at::Tensor& labels) {
+    const Answers a = check_answers(logits, labels);
+    const auto opt = logits.options().dtype(at::kFloat);
+    at::Tensor logps = at::empty(labels.sizes(), opt), stats = at::empty({a.B, a.S, 2}, opt);
+    if (labels.numel() == 0) return {logps, stats};
+    Launch L(logits.device());
+    const int rc = q4_token_logps(a.logits.data_ptr(), a.type, a.logits.stride(0), a.logits.stride(1), (int)a.B, (int)a.S, (int)a.V, a.label_ptr(),
+                                  logps.data_ptr<float>(), stats.data_ptr<float>(), L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_token_logps");
+    return {logps, stats};
+}
+
+at::Tensor token_logps_bwd(const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& stats, const at::Tensor& coef, const c10::optional<at::Tensor>& factor) {
+    const Answers a = check_answers(logits, labels);
+    TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat && stats.dim() == 3 && stats.size(0) == a.B && stats.size(1) == a.S && stats.size(2) == 2 && stats.is_contiguous() &&
+                      stats.device() == logits.device(), "stats must be what token_logps gave for these logits");
+    TORCH_CHECK_VALUE(coef.scalar_type() == at::kFloat && coef.device() == logits.device() && (coef.sizes() == labels.sizes() || (coef.dim() == 1 && coef.size(0) == a.B)),
+                      "coef must be a float32 tensor on the logits' device, one for each place or one for each sequence");
+    TORCH_CHECK_VALUE(!factor.has_value() || (factor->scalar_type() == at::kFloat && factor->numel() == 1 && factor->device() == logits.device()),
+                      "factor must be one float32 on the logits' device");
+    check_no_grad(stats, "stats");
+    check_no_grad(coef, "coef");
+    if (factor.has_value()) check_no_grad(*factor, "factor");
+    const at::Tensor c = coef.contiguous();
+    at::Tensor dx = at::empty(logits.sizes(), logits.options());
+    if (labels.numel() == 0) return dx;
+    const int per = coef.sizes() == labels.sizes() ? 1 : (int)a.S;
+    Launch L(logits.device());
+    const int rc = q4_token_logps_bwd(a.logits.data_ptr(), a.type, a.logits.stride(0), a.logits.stride(1), (int)a.B, (int)a.S, (int)a.V, a.label_ptr(),
+                                      stats.data_ptr<float>(), c.data_ptr<float>(), per, factor.has_value() ? factor->data_ptr<float>() : nullptr, dx.data_ptr(), L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_token_logps_bwd");
+    return dx;
+}
+
+// (loss [], rewards [2P], coef [2P], stats)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> preference_loss(const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& ref_logps, double beta,
+                                                                           double smoothing) {
+    TORCH_CHECK_VALUE(logits.dim() == 3, "logits must be a [2P, S, V] tensor on the GPU");
+    const Answers a = check_answers(logits, labels);
+    TORCH_CHECK_VALUE(a.B >= 2 && a.B % 2 == 0 && a.S >= 1, "a call takes whole pairs of at least one place; got ", a.B, " sequences of ", a.S);
+    TORCH_CHECK_VALUE(ref_logps.scalar_type() == at::kFloat && ref_logps.sizes() == labels.sizes() && ref_logps.device() == logits.device(),
+                      "ref_logps must be a float32 [2P, S] tensor on the logits' device");
+    TORCH_CHECK_VALUE(beta > 0.0 && std::isfinite(beta), "beta must be positive and finite");
+    TORCH_CHECK_VALUE(smoothing >= 0.0 && smoothing <= 0.5, "label_smoothing must be in [0, 0.5]");
+    check_no_grad(ref_logps, "ref_logps");
+    const at::Tensor r = ref_logps.contiguous();
+    const auto opt = logits.options().dtype(at::kFloat);
+    at::Tensor loss = at::empty({}, opt), rewards = at::empty({a.B}, opt), coef = at::empty({a.B}, opt), stats = at::empty({a.B, a.S, 2}, opt);
+    const size_t need = q4_preference_loss_workspace_bytes((int)(a.B / 2), (int)a.S);
+    at::Tensor ws = at::empty({(int64_t)need}, opt.dtype(at::kByte));
+    Launch L(logits.device());
+    const int rc = q4_preference_loss(a.logits.data_ptr(), a.type, a.logits.stride(0), a.logits.stride(1), (int)(a.B / 2), (int)a.S, (int)a.V, a.label_ptr(),
+                                      r.data_ptr<float>(), beta, smoothing, loss.data_ptr<float>(), rewards.data_ptr<float>(), coef.data_ptr<float>(),
+                                      stats.data_ptr<float>(), ws.data_ptr(), need, L.stream);
+    if (rc != Q4_OK) raise_q4(rc, "q4_preference_loss");
+    return {loss, rewards, coef, stats};
+}
+
+// The two as functions of autograd.  A graph of the backward pass (create_graph) is refused by check_no_grad, as is forward mode by autograd itself.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct TokenLogps : torch::autograd::Function<TokenLogps> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels) {
+        auto r = token_logps(logits, labels);
+        ctx->save_for_backward({logits, labels, r.second});
+        return r.first;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        return {token_logps_bwd(saved[0], saved[1], saved[2], grads[0], c10::nullopt), at::Tensor()};
+    }
+};
+
+struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& ref_logps, double beta, double smoothing) {
+        auto r = preference_loss(logits, labels, ref_logps, beta, smoothing);
+        ctx->save_for_backward({logits, labels, std::get<3>(r), std::get<2>(r)});
+        ctx->mark_non_differentiable({std::get<1>(r)});
+        return {std::get<0>(r), std::get<1>(r)};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        return {token_logps_bwd(saved[0], saved[1], saved[2], saved[3], grads[0]), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+at::Tensor token_logps_autograd(const at::Tensor& logits, const at::Tensor& labels) { return TokenLogps::apply(logits, labels); }
+
+std::pair<at::Tensor, at::Tensor> preference_loss_autograd(const at::Tensor& logits, const at::Tensor& labels, const at::Tensor& ref_logps, double beta, double smoothing) {
+    check_no_grad(ref_logps, "ref_logps");                                   // the reference is not trained
+    auto r = PreferenceLoss::apply(logits, labels, ref_logps, beta, smoothing);
+    return {r[0], r[1]};
+}
+
 // True when the cached GEMV accumulators of every stream are all zero (synchronises; for tests and debugging).
 bool workspaces_are_zero() {
     std::lock_guard<std::mutex> lock(g_mutex);
@@ -989,6 +1203,15 @@ PYBIND11_MODULE(_q4_host, m) {
     m.def("kv4_attention", &kv4_attention, py::arg("q"), py::arg("cache"), py::arg("page_table"), py::arg("lengths"), py::arg("scale") = 0.0,
           py::arg("starts") = py::none(), py::arg("max_tokens") = py::none(), py::arg("max_length") = py::none(), py::arg("out") = py::none());
     m.def("lora_rows", &lora_rows, py::arg("x"), py::arg("index"), py::arg("specs"), py::arg("per") = 1);
+    m.def("act8_pack", &act8_pack, py::arg("x"));
+    m.def("act8_unpack", &act8_unpack, py::arg("codes"), py::arg("scales"), py::arg("dtype"));
+    m.def("silu_mul_act8", &silu_mul_act8, py::arg("gate"), py::arg("up"));
+    m.def("silu_mul_act8_bwd", &silu_mul_act8_bwd, py::arg("dout"), py::arg("kept"));
+    m.def("token_logps", &token_logps, py::arg("logits"), py::arg("labels"));
+    m.def("token_logps_bwd", &token_logps_bwd, py::arg("logits"), py::arg("labels"), py::arg("stats"), py::arg("coef"), py::arg("factor") = py::none());
+    m.def("preference_loss", &preference_loss, py::arg("logits"), py::arg("labels"), py::arg("ref_logps"), py::arg("beta"), py::arg("smoothing"));
+    m.def("token_logps_autograd", &token_logps_autograd, py::arg("logits"), py::arg("labels"));
+    m.def("preference_loss_autograd", &preference_loss_autograd, py::arg("logits"), py::arg("labels"), py::arg("ref_logps"), py::arg("beta"), py::arg("smoothing"));
     m.def("mlp_decode_gave_up", &mlp_decode_gave_up);
     m.def("reset_workspaces", &reset_workspaces);
     m.def("workspaces_are_zero", &workspaces_are_zero);

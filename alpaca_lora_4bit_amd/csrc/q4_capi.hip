@@ -79,7 +79,7 @@ int check_layer(const void* qweight, const void* qzeros, const void* scales, con
 }
 }  // namespace
 
-extern "C" int q4_abi_version(void) { return 19; }
+extern "C" int q4_abi_version(void) { return 20; }
 
 extern "C" const char* q4_error_string(int code) {
     switch (code) {

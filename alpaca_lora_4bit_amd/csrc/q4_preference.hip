@@ -1,0 +1,355 @@
+// Log-probabilities of the tokens of answers from logits, their gradient, and the loss of pairs of answers (paired log ratios).
+//
+//   logp = (x_l - m) - log(sum of exp(x - m)) for any m        dx = c (1[l] - exp(x - m - log sum))
+//
+// HBM-bound: one pass over a row's logits, backward one pass more from the two numbers (m, log sum) that forward left.  Rows whose label is not one of the V words are no tokens of an answer (a prompt,
+// padding): they are not read, and their gradient is zero.  Exponentials and a lane's sum in fp32, what follows in fp64: a log ratio is the small
+// difference of sums of some hundred log-probabilities, and an error in one direction grows with the answer.
+#include "q4_common.hpp"
+#include "q4_gptq.h"
+#include "q4_preference.hpp"
+
+namespace q4 {
+
+constexpr float kLog2eHi = 0x1.715476p+0f, kLog2eLo = 0x1.4ae0c0p-26f;       // log2(e) in two parts
+constexpr double kExpShort = 3e-9;                                           // v_exp_f32 is short by so much of itself on average (measured: sum of 4 million)
+
+// exp(d) for d <= 0.  With one fp32 factor log2(e) every exponent is short by 1.3e-8 of itself: all in one direction, which a log ratio over a
+// long answer adds up.
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(fmaf(d, kLog2eHi, d * kLog2eLo)); }
+
+template <typename T>
+struct Pack {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+template <typename T>
+__device__ __forceinline__ Pack<T> load_pack(const T* p) { return __builtin_bit_cast(Pack<T>, *reinterpret_cast<const uint4_t*>(p)); }
+template <typename T>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T>& r) { *reinterpret_cast<uint4_t*>(p) = __builtin_bit_cast(uint4_t, r); }
+
+// Values before the first 16-byte boundary of a row, packs behind it, values left.
+template <typename T>
+struct Split {
+    int head, packs, tail;
+    __device__ __forceinline__ Split(const T* row, int V) {
+        const int to = (int)((0u - (unsigned)reinterpret_cast<uintptr_t>(row)) & 15u) / (int)sizeof(T);
+        head = to < V ? to : V;
+        packs = (V - head) / Pack<T>::N;
+        tail = V - head - packs * Pack<T>::N;
+    }
+};
+
+// Sum of exp(x - at) of a lane's values.  Those of a pack are added up first, and their sum with what the addition before lost (Kahan): beside a
+// word that has most of the weight the many small ones would each lose half a unit of it.
+struct Sum {
+    float s = 0.f, lost = 0.f;
+    template <typename T, int N>
+    __device__ __forceinline__ void add(const T (&x)[N], float at) {
+        float part[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) part[e] = exp_of((float)x[e] - at);
+#pragma unroll
+        for (int w = N / 2; w >= 1; w /= 2)
+#pragma unroll
+            for (int e = 0; e < w; ++e) part[e] += part[e + w];
+        const float old = s, more = part[0] - lost;
+        s = old + more;
+        lost = (s - old) - more;
+    }
+};
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const LogitsView& a, long row) {
+    const long b = row / a.S, t = row - b * a.S;
+    return reinterpret_cast<const T*>(a.x) + b * a.sb + t * a.st;
+}
+
+template <int WAVES>
+__device__ __forceinline__ float group_max(float v, float* lds) {
+    v = wave_max(v);
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v = fmaxf(v, lds[w]);
+    }
+    return v;
+}
+template <int WAVES>
+__device__ __forceinline__ double group_sum(double v, double* lds) {
+    v = wave_sum(v);
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+        __syncthreads();
+        v = 0.0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v += lds[w];
+    }
+    return v;
+}
+
+// A row's sum of exp(x - at), at = the label's own logit: exponents need no maximum first, and what follows is -log(sum).  Where the label's logit is
+// so far below others that this leaves fp32 (by 80 and more), is no number, or the row has an infinity, the row is read again for its maximum and once more
+// for the sum beside it.  `logps` or `wide` (the other is null) takes the log-probability: in fp32 for a caller, in fp64 for the log ratios.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_logps_kernel(LogitsView a, const long long* __restrict__ labels, float* __restrict__ logps, double* __restrict__ wide,
+                                                              float2* __restrict__ stats) {
+    constexpr int N = Pack<T>::N, WAVES = THREADS / 64, U = 4;
+    __shared__ float sm[WAVES];
+    __shared__ double ss[WAVES];
+    const int tid = threadIdx.x;
+    const long rows = (long)a.B * a.S;
+    for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const long long label = labels[row];
+        if (label < 0 || label >= a.V) {
+            if (tid == 0) {
+                if (logps) logps[row] = 0.f;
+                else wide[row] = 0.0;
+                stats[row] = float2{0.f, 0.f};
+            }
+            continue;
+        }
+        const T* x = row_of<T>(a, row);
+        const float mine = (float)x[label];
+        const Split<T> sp(x, a.V);
+        const T* body = x + sp.head;
+        Sum r;
+        for (int i = tid; i < sp.packs; i += U * THREADS) {
+            Pack<T> p[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {                                    // all on their way, the ones behind the end from the last place
+                const int k = i + u * THREADS;
+                p[u] = load_pack(body + (long)(k < sp.packs ? k : sp.packs - 1) * N);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u * THREADS < sp.packs) r.add(p[u].v, mine);
+        }
+        if (tid < sp.head) { const T one[1] = {x[tid]}; r.add(one, mine); }
+        if (tid < sp.tail) { const T one[1] = {body[(long)sp.packs * N + tid]}; r.add(one, mine); }
+        double s = group_sum<WAVES>((double)r.s - (double)r.lost, ss);
+        float at = mine;
+        if (!(s < 0x1p115)) {                                                // the same in all threads
+            at = -0x1.FFFFFEp127f;                                           // rows of this number or of -infinity give what their definition gives
+            for (long i = tid; i < a.V; i += THREADS) at = fmaxf(at, (float)x[i]);
+            at = group_max<WAVES>(at, sm);
+            Sum again;
+            for (long i = tid; i < a.V; i += THREADS) { const T one[1] = {x[i]}; again.add(one, at); }
+            s = group_sum<WAVES>((double)again.s - (double)again.lost, ss);
+        }
+        if (tid == 0) {
+            // one term of the sum, exp(0), is exact; the fp32 logarithm would be 3e-7 short on average
+            const double total = log(s + kExpShort * (s - 1.0)), lp = ((double)mine - (double)at) - total;
+            if (logps) logps[row] = (float)lp;
+            else wide[row] = lp;
+            stats[row] = float2{at, (float)total};
+        }
+    }
+}
+
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_logps_bwd_kernel(LogitsView a, const long long* __restrict__ labels, const float2* __restrict__ stats,
+                                                                  const float* __restrict__ coef, int per, const float* __restrict__ factor, T* __restrict__ dx) {
+    constexpr int N = Pack<T>::N, U = 4;
+    const int tid = threadIdx.x;
+    const long rows = (long)a.B * a.S;
+    for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const long long label = labels[row];
+        T* out = dx + row * a.V;
+        if (label < 0 || label >= a.V) {
+            const Split<T> so(out, a.V);
+            Pack<T> zero;
+#pragma unroll
+            for (int e = 0; e < N; ++e) zero.v[e] = (T)0.f;
+            for (int i = tid; i < so.packs; i += THREADS) store_pack(out + so.head + (long)i * N, zero);
+            if (tid < so.head) out[tid] = (T)0.f;
+            if (tid < so.tail) out[so.head + (long)so.packs * N + tid] = (T)0.f;
+            continue;
+        }
+        const T* x = row_of<T>(a, row);
+        const float2 st = stats[row];
+        const float c = (factor ? *factor : 1.f) * coef[row / per];
+        auto share = [&](T v) { return (T)(-c * __expf(((float)v - st.x) - st.y)); };
+        // the label's own gradient c (1 - p), formed without that difference
+        auto own = [&](T v) { return (T)(-c * expm1f(((float)v - st.x) - st.y)); };
+        const Split<T> sp(x, a.V);
+        if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0) {
+            for (int i = tid; i < sp.packs; i += U * THREADS) {
+                Pack<T> p[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int k = i + u * THREADS;
+                    p[u] = load_pack(x + sp.head + (long)(k < sp.packs ? k : sp.packs - 1) * N);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (i + u * THREADS >= sp.packs) break;
+                    const long at = sp.head + (long)(i + u * THREADS) * N;
+                    Pack<T> g;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) g.v[e] = share(p[u].v[e]);
+                    if ((unsigned long)(label - at) < N) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e)
+                            if (label == at + e) g.v[e] = own(p[u].v[e]);
+                    }
+                    store_pack(out + at, g);
+                }
+            }
+            if (tid < sp.head) out[tid] = tid == label ? own(x[tid]) : share(x[tid]);
+            const long at = sp.head + (long)sp.packs * N + tid;
+            if (tid < sp.tail) out[at] = at == label ? own(x[at]) : share(x[at]);
+        } else {                                                             // strides that put x and dx at different places of 16 bytes
+            for (long i = tid; i < a.V; i += THREADS) out[i] = i == label ? own(x[i]) : share(x[i]);
+        }
+    }
+}
+
+constexpr int kRatioThreads = 256, kPairThreads = 1024;
+
+// This thread's share of an answer's log ratio, threads apart; four places on their way.
+__device__ __forceinline__ double ratio_share(const double* __restrict__ logps, const float* __restrict__ ref, const long long* __restrict__ labels, int S, int V, int first,
+                                              int apart) {
+    double sum = 0.0;
+    for (int t = first; t < S; t += 4 * apart) {
+        long long l[4];
+        double x[4];
+        float y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int k = t + u * apart < S ? t + u * apart : S - 1;
+            l[u] = t + u * apart < S ? labels[k] : -1;
+            x[u] = logps[k];
+            y[u] = ref[k];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (l[u] >= 0 && l[u] < V) sum += x[u] - (double)y[u];           // what the reference says elsewhere is not looked at
+    }
+    return sum;
+}
+
+__global__ __launch_bounds__(kRatioThreads) void answer_ratio_kernel(const double* __restrict__ logps, const float* __restrict__ ref, const long long* __restrict__ labels,
+                                                                     int B, int S, int V, double* __restrict__ ratios) {
+    __shared__ double lds[kRatioThreads / 64];
+    for (int b = blockIdx.x; b < B; b += gridDim.x) {
+        const long base = (long)b * S;
+        const double r = group_sum<kRatioThreads / 64>(ratio_share(logps + base, ref + base, labels + base, S, V, threadIdx.x, kRatioThreads), lds);
+        if (threadIdx.x == 0) ratios[b] = r;
+    }
+}
+
+// One workgroup: the pairs' losses, their mean, and what the gradient of the mean with respect to each answer's log-probabilities is.  SUMS: also
+// the answers' log ratios, a wavefront an answer.
+template <bool SUMS>
+__global__ __launch_bounds__(kPairThreads) void preference_pairs_kernel(const double* __restrict__ logps, const float* __restrict__ ref, const long long* __restrict__ labels,
+                                                                        int P, int S, int V, double beta, double smoothing, double* ratios, float* __restrict__ loss,
+                                                                        float* __restrict__ rewards, float* __restrict__ coef) {
+    __shared__ double lds[kPairThreads / 64];
+    if constexpr (SUMS) {
+        for (int b = threadIdx.x / 64; b < 2 * P; b += kPairThreads / 64) {
+            const long base = (long)b * S;
+            const double r = wave_sum(ratio_share(logps + base, ref + base, labels + base, S, V, threadIdx.x % 64, 64));
+            if (threadIdx.x % 64 == 0) ratios[b] = r;
+        }
+        __syncthreads();
+    }
+    double sum = 0.0;
+    for (int p = threadIdx.x; p < P; p += kPairThreads) {
+        const double good = ratios[p], bad = ratios[p + P], z = beta * (good - bad);
+        const double e = exp(-fabs(z)), soft = log1p(e), sure = 1.0 / (1.0 + e);
+        const double pos = z >= 0.0 ? sure : e * sure, neg = z >= 0.0 ? e * sure : sure;      // sigmoid(z), sigmoid(-z)
+        double one = (1.0 - smoothing) * (soft + fmax(-z, 0.0));
+        if (smoothing > 0.0) one += smoothing * (soft + fmax(z, 0.0));       // z may be infinite
+        const double dz = (smoothing * pos - (1.0 - smoothing) * neg) * (beta / P);
+        rewards[p] = (float)(beta * good);
+        rewards[p + P] = (float)(beta * bad);
+        coef[p] = (float)dz;
+        coef[p + P] = (float)-dz;
+        sum += one;
+    }
+    sum = group_sum<kPairThreads / 64>(sum, lds);
+    if (threadIdx.x == 0) *loss = (float)(sum / P);
+}
+
+constexpr long kMostGroups = 1 << 20;                                        // workgroups of a launch; they go on to further rows
+
+template <typename F>
+int by_type(int type, F&& launch) {
+    switch (type) {
+        case Q4_TYPE_F16: launch((half_t)0.f); break;
+        case Q4_TYPE_BF16: launch((__bf16)0.f); break;
+        default: launch(0.f); break;
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -4;
+}
+
+}  // namespace q4
+
+// Threads of a row's workgroup.  Wavefronts by themselves for rows of up to 4 KB (32768 rows of 640 bytes, forward / backward: 64 threads 15 / 17 us,
+// 256 34 / 39).  Forward 256, and 512 where there are few rows or long ones (37 rows of 64 KB: 7.6 against 8.5 us, 2048 of 256 KB 96 against 110; 1024 threads
+// wait for each other: 32768 rows of 64 KB 415 against 199).  Backward, where nothing waits, 1024 for rows of 48 KB and more (the same rows 587 against 626).
+namespace {
+template <typename F>
+void by_width(bool forward, long rows, long bytes, F&& launch) {
+    const dim3 grid((unsigned)(rows < q4::kMostGroups ? rows : q4::kMostGroups));
+    if (bytes <= 4096) launch(std::integral_constant<int, 64>{}, grid);
+    else if (forward && (rows <= 512 || bytes >= 192 * 1024)) launch(std::integral_constant<int, 512>{}, grid);
+    else if (!forward && bytes >= 48 * 1024) launch(std::integral_constant<int, 1024>{}, grid);
+    else launch(std::integral_constant<int, 256>{}, grid);
+}
+}  // namespace
+
+int q4_launch_token_logps(const q4::LogitsView& a, int type, const long long* labels, float* logps, double* wide, float* stats, hipStream_t stream) {
+    using namespace q4;
+    return by_type(type, [&](auto t) {
+        using T = decltype(t);
+        by_width(true, (long)a.B * a.S, (long)a.V * sizeof(T), [&](auto threads, dim3 grid) {
+            constexpr int TH = decltype(threads)::value;
+            if constexpr (TH < 1024)
+                hipLaunchKernelGGL((token_logps_kernel<T, TH>), grid, dim3(TH), 0, stream, a, labels, logps, wide, (float2*)stats);
+        });
+    });
+}
+
+int q4_launch_token_logps_bwd(const q4::LogitsView& a, int type, const long long* labels, const float* stats, const float* coef, int per, const float* factor,
+                              void* dx, hipStream_t stream) {
+    using namespace q4;
+    return by_type(type, [&](auto t) {
+        using T = decltype(t);
+        by_width(false, (long)a.B * a.S, (long)a.V * sizeof(T), [&](auto threads, dim3 grid) {
+            constexpr int TH = decltype(threads)::value;
+            if constexpr (TH != 512)
+                hipLaunchKernelGGL((token_logps_bwd_kernel<T, TH>), grid, dim3(TH), 0, stream, a, labels, (const float2*)stats, coef, per, factor, (T*)dx);
+        });
+    });
+}
+
+int q4_launch_preference_pairs(const double* logps, const float* ref, const long long* labels, int P, int S, int V, double beta, double smoothing, float* loss,
+                               float* rewards, float* coef, double* ratios, hipStream_t stream) {
+    using namespace q4;
+    // One launch where a wavefront has one or two answers of 256 places to add up (us, one / two launches: 1 pair of 48 places 3.6 / 5.3, 16 of 256
+    // 5.8 / 6.0, 4 of 2048 7.6 / 5.9, 16 of 1024 11.9 / 5.8).
+    if ((2l * P + 15) / 16 * ((S + 255l) / 256) <= 2) {
+        hipLaunchKernelGGL(preference_pairs_kernel<true>, dim3(1), dim3(kPairThreads), 0, stream, logps, ref, labels, P, S, V, beta, smoothing, ratios, loss, rewards, coef);
+    } else {
+        const unsigned groups = (unsigned)(2l * P < kMostGroups ? 2l * P : kMostGroups);
+        hipLaunchKernelGGL(answer_ratio_kernel, dim3(groups), dim3(kRatioThreads), 0, stream, logps, ref, labels, 2 * P, S, V, ratios);
+        hipLaunchKernelGGL(preference_pairs_kernel<false>, dim3(1), dim3(kPairThreads), 0, stream, logps, ref, labels, P, S, V, beta, smoothing, ratios, loss, rewards, coef);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -4;
+}

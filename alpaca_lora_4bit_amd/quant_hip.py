@@ -1077,6 +1077,56 @@ def lora_rows(x, index, specs, rows_per_index=1):
     _serving().lora_rows(x, index, specs, int(rows_per_index))
 
 
+# ------------------------------------------------------------------------- training: what a step keeps, and the loss of pairs of answers
+# Activations in 8 bits: of every 32 neighbouring values (in the order of a contiguous tensor, whatever its shape) the scale s is the least bfloat16
+# with 127 s >= their largest magnitude, and a value is held as the nearest whole number of s (ties to the even one), off by s / 2 at most.  32 values of
+# which one is an infinity or NaN read back as NaN.  These calls know no gradients (a call whose inputs require grad under grad mode is refused): the
+# differentiable ones are preference.token_logps, preference.preference_loss and what model_attn_mlp_patch and gradient_checkpointing put in place.
+def _training():
+    _require(_host is not None, "the training operators need the compiled host binding (_q4_host)")
+    return _host
+
+
+def act8_pack(x):
+    """(codes int8 of x's shape, scales bfloat16 [ceil(n / 32)]) of x fp16, bf16 or fp32."""
+    return _training().act8_pack(x)
+
+
+def act8_unpack(codes, scales, dtype=torch.float16):
+    """The values that codes and scales stand for, rounded to `dtype` (fp16, bf16 or fp32; not beyond its largest number)."""
+    return _training().act8_unpack(codes, scales, dtype)
+
+
+def silu_mul_act8(gate, up):
+    """(silu(gate) * up, kept) for gate, up fp16 or bf16 of one shape; the product is formed in fp32 and rounded once, and kept = (gate's codes, gate's
+    scales, up's codes, up's scales) as act8_pack gives them."""
+    return _training().silu_mul_act8(gate, up)
+
+
+def silu_mul_act8_bwd(dout, kept):
+    """(dgate, dup) of silu(gate) * up in dout's type (fp16 or bf16), at the values that `kept` holds."""
+    return _training().silu_mul_act8_bwd(dout, kept)
+
+
+def token_logps(logits, labels):
+    """(logps, stats): logps fp32 of labels' shape = log softmax(logits)[label] for logits [..., V] (fp16, bf16, fp32; any strides) and int64 labels [...],
+    0 where a label is not one of 0 .. V - 1 (the logits there are not read); stats is for token_logps_bwd."""
+    return _training().token_logps(logits, labels)
+
+
+def token_logps_bwd(logits, labels, stats, coef, factor=None):
+    """factor * coef * (1[label] - softmax(logits)) in logits' type and shape, zero where the label is no word; coef fp32 for each place, or one for each of
+    the sequences of 3-D logits; factor one fp32 on the device (None: 1)."""
+    return _training().token_logps_bwd(logits, labels, stats, coef, factor)
+
+
+def preference_loss(logits, labels, ref_logps, beta, label_smoothing=0.0):
+    """(loss, rewards, coef, stats) of P pairs: logits [2P, S, V] and int64 labels [2P, S] as above, ref_logps fp32 [2P, S], sequence p preferred to
+    sequence p + P.  With r the sums of log-probability - ref_logps over the places whose label is a word and z = beta (r[:P] - r[P:]): loss [] = mean of
+    -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z), rewards [2P] = beta r, coef [2P] = dloss / dr and stats for token_logps_bwd."""
+    return _training().preference_loss(logits, labels, ref_logps, float(beta), float(label_smoothing))
+
+
 # ------------------------------------------------- quant_cuda-compatible entry points
 def _infer_groupsize(K, G):
     return -(-K // G)

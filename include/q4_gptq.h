@@ -422,6 +422,43 @@ Q4_API size_t q4_lora_rows_workspace_bytes(int count, int M, int K, int R);
 Q4_API int q4_lora_rows_f16(const q4_lora_rows_t *probs, int count, const void *x, const int32_t *index, int per, int M, int K, int R, int n,
                      void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- training on pairs of answers, and what a step keeps for its backward pass ------------------------------------------
+ * The type of a call's floating tensors. */
+#define Q4_TYPE_F16 0
+#define Q4_TYPE_BF16 1
+#define Q4_TYPE_F32 2
+/* n values in 8 bits: in blocks of 32 neighbours (the last one as short as it comes) value = code * scale, codes int8 [n], scales bfloat16 [(n + 31) / 32].
+ * The scale is the least bfloat16 s with 127 s >= the block's largest magnitude, a code the nearest whole number of s (ties to the even one), so that a value
+ * is off by at most s / 2.  A block with an infinity or NaN reads back as NaN.  No counterpart in the reference, whose checkpoints hold the blocks' inputs as
+ * they are (gradient_checkpointing.py:17-31).  1 <= n < 2^35 - 2048; all pointers 16-byte aligned. */
+typedef struct { void *codes, *scales; } q4_act8_t;
+Q4_API int q4_act8_pack(const void *x, int type, void *codes, void *scales, long long n, void *stream);
+/* x = code * scale, rounded to `type` (which need not be the packed one) and no further out than its largest number. */
+Q4_API int q4_act8_unpack(const void *codes, const void *scales, void *x, int type, long long n, void *stream);
+
+/* out = silu(gate) * up (model_attn_mlp_patch.py:224-228) from fp16 or bfloat16 gate, up [n], formed in fp32 and rounded once; both are kept in 8 bits.
+ * Backward from what was kept: dup = dout * gate * s, dgate = dout * up * s * (1 + gate * (1 - s)) with s = sigmoid(gate).  n and alignment as above. */
+Q4_API int q4_silu_mul_act8(const void *gate, const void *up, int type, void *out, const q4_act8_t *kept_gate, const q4_act8_t *kept_up, long long n, void *stream);
+Q4_API int q4_silu_mul_act8_bwd(const void *dout, int type, const q4_act8_t *kept_gate, const q4_act8_t *kept_up, void *dgate, void *dup, long long n, void *stream);
+
+/* logps fp32 [B, S] = log softmax(logits [B, S, V])[label] with labels int64 [B, S]; a label outside 0 .. V - 1 is no token: its logits are not read and its logps
+ * are 0.  Logits: strides sb, st >= 0 in elements, a row's V values side by side.  stats fp32 [B, S, 2]: what the backward pass takes.  B * S <= 2^31 - 1, V < 2^30.
+ * An infinity among a row's logits counts as in softmax: -infinity as no weight, +infinity makes the row NaN.  The reference's only loss is the host model's
+ * next-token loss (finetune.py:126-180). */
+Q4_API int q4_token_logps(const void *logits, int type, long long sb, long long st, int B, int S, int V, const long long *labels, float *logps, float *stats, void *stream);
+/* dlogits [B, S, V] (contiguous, the logits' type) = factor * coef[row / per] * (1[v == label] - softmax(logits)), zero where the label is no token; coef fp32
+ * [B * S / per] (per divides B * S), factor one fp32 in device memory or NULL for 1. */
+Q4_API int q4_token_logps_bwd(const void *logits, int type, long long sb, long long st, int B, int S, int V, const long long *labels, const float *stats, const float *coef,
+                       int per, const float *factor, void *dlogits, void *stream);
+/* P pairs in logits [2P, S, V]: sequences p (preferred) and p + P (rejected).  r_b = sum over the tokens (labels as above) of log-probability - ref, ref fp32
+ * [2P, S], not used where the label is no token; z_p = beta * (r_p - r_{p+P}); loss = mean over p of -(1 - smoothing) log sigmoid(z_p) - smoothing
+ * log sigmoid(-z_p); rewards fp32 [2P] = beta * r; coef fp32 [2P] = dloss / dr, what q4_token_logps_bwd takes with per = S, stats as there.  Log-probabilities,
+ * their sums (in a fixed order) and the loss in fp64.  beta > 0 and finite, 0 <= smoothing <= 0.5.  `workspace`: the bytes that the query gives, 8-byte aligned,
+ * contents irrelevant. */
+Q4_API size_t q4_preference_loss_workspace_bytes(int P, int S);
+Q4_API int q4_preference_loss(const void *logits, int type, long long sb, long long st, int P, int S, int V, const long long *labels, const float *ref, double beta,
+                       double smoothing, float *loss, float *rewards, float *coef, float *stats, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
