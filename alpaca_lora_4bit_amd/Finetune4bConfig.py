@@ -13,7 +13,7 @@ _PLAIN_FIELDS = (
     "llama_q4_model", "mbatch_size", "batch_size", "epochs", "lr", "cutoff_len", "lora_r", "lora_alpha",
     "gradient_checkpointing", "gradient_checkpointing_ratio", "warmup_steps", "save_steps", "save_total_limit",
     "logging_steps", "checkpoint", "skip", "verbose", "txt_row_thd", "use_eos_token", "groupsize", "v1",
-    "flash_attention", "xformers", "backend",
+    "flash_attention", "xformers", "backend", "act_bits", "beta", "label_smoothing",
 )
 
 # sections of the printed summary: (title, attributes)
@@ -22,18 +22,20 @@ _SUMMARY = (
     ("training", ("mbatch_size", "batch_size", "gradient_accumulation_steps", "epochs", "lr", "cutoff_len", "lora_r",
                   "lora_alpha", "lora_dropout", "val_set_size", "gradient_checkpointing",
                   "gradient_checkpointing_ratio", "warmup_steps", "save_steps", "save_total_limit", "logging_steps",
-                  "checkpoint", "skip", "world_size", "ddp", "device_map", "groupsize", "v1", "backend")),
+                  "checkpoint", "skip", "world_size", "ddp", "device_map", "groupsize", "v1", "backend", "act_bits", "beta",
+                  "label_smoothing")),
 )
 
 
 class Finetune4bConfig:
-    """Config holder for 4-bit LLaMA LoRA finetuning; keyword arguments as in the reference (`:5-20`)."""
+    """Config holder for 4-bit LLaMA LoRA finetuning; keyword arguments as in the reference (`:5-20`) and three of its own: `act_bits` (8: checkpoints and
+    the MLP blocks' activations in 8 bits), `beta` and `label_smoothing` (preference loss)."""
 
     def __init__(self, dataset, ds_type, lora_out_dir, lora_apply_dir, resume_checkpoint, llama_q4_config_dir,
                  llama_q4_model, mbatch_size, batch_size, epochs, lr, cutoff_len, lora_r, lora_alpha, lora_dropout,
                  val_set_size, gradient_checkpointing, gradient_checkpointing_ratio, warmup_steps, save_steps,
                  save_total_limit, logging_steps, checkpoint, skip, verbose, txt_row_thd, use_eos_token, groupsize,
-                 v1, local_rank, flash_attention, xformers, backend):
+                 v1, local_rank, flash_attention, xformers, backend, act_bits=16, beta=0.1, label_smoothing=0.0):
         given = locals()
         for name in _PLAIN_FIELDS:
             setattr(self, name, given[name])

@@ -2,6 +2,8 @@
 reference's src/alpaca_lora_4bit/arg_parser.py:5-80, returned as a `Finetune4bConfig` by `get_config()`
 (`:83-117`; its `finetune.py:23-24` calls that before anything else is imported).
 
+Options that the reference lacks (`--act_bits`, `--beta`, `--label_smoothing`) are in the result only where they are given.
+
 `--backend` keeps its two spellings; both select the HIP kernels here (see `autograd_4bit.switch_backend_to`).
 """
 import argparse
@@ -12,7 +14,7 @@ from .Finetune4bConfig import Finetune4bConfig
 # (group, flags, argparse keywords); help texts are generated from the defaults
 _CONFIG, _TRAINING = "config", "training"
 _OPTIONS = (
-    (_CONFIG, ("--ds_type",), dict(choices=["txt", "alpaca", "gpt4all", "bluemoon"], default="alpaca",
+    (_CONFIG, ("--ds_type",), dict(choices=["txt", "alpaca", "gpt4all", "bluemoon", "preference"], default="alpaca",
                                    help="Dataset structure format")),
     (_CONFIG, ("--lora_out_dir",), dict(default="alpaca_lora", help="Directory to place new LoRA")),
     (_CONFIG, ("--lora_apply_dir",), dict(default=None, help="Directory of a LoRA to apply before training")),
@@ -46,6 +48,10 @@ _OPTIONS = (
     (_TRAINING, ("--flash_attention",), dict(action="store_true", help="Use the flash-attention patch")),
     (_TRAINING, ("--xformers",), dict(action="store_true", help="Use the xformers attention patch")),
     (_TRAINING, ("--backend",), dict(default="cuda", type=str, help="Kernel backend name: cuda or triton")),
+    (_TRAINING, ("--act_bits",), dict(default=argparse.SUPPRESS, type=int, choices=[8, 16], help="8: checkpoints and the MLP blocks' activations are kept in 8 bits "
+                                      "for the backward pass. Default: 16, as they are")),
+    (_TRAINING, ("--beta",), dict(default=argparse.SUPPRESS, type=float, help="Preference loss: factor of the log ratios. Default: 0.1")),
+    (_TRAINING, ("--label_smoothing",), dict(default=argparse.SUPPRESS, type=float, help="Preference loss: share of pairs taken to be the wrong way round. Default: 0")),
 )
 
 # argparse destination -> Finetune4bConfig keyword where the two differ
@@ -59,7 +65,8 @@ def _build_parser() -> argparse.ArgumentParser:
     groups = {name: parser.add_argument_group(name) for name in (_CONFIG, _TRAINING)}
     for group, flags, kw in _OPTIONS:
         kw = dict(kw)
-        kw["help"] = kw["help"] + ". Default: %(default)s"
+        if kw.get("default") is not argparse.SUPPRESS:
+            kw["help"] = kw["help"] + ". Default: %(default)s"
         groups[group].add_argument(*flags, required=False, **kw)
     return parser
 

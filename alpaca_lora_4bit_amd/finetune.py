@@ -14,6 +14,10 @@ file layout (`adapter_config.json` + `adapter_model.safetensors`, keys `base_mod
 so that peft can read it later.  wandb is used when importable (finetune.py:183), skipped otherwise.
 The flash-attention / xformers attention patches of the reference are not part of this package; their flags are
 accepted and ignored with a note.
+
+Two additions: `--ds_type preference` trains on records of a prompt, a preferred and a rejected answer with the preference loss (preference.py; `--beta`,
+`--label_smoothing`), the reference being the model without its adapters; `--act_bits 8` keeps the checkpoints of `--grad_chckpt` and the outputs of
+gate_proj and up_proj in 8 bits for the backward pass.
 """
 import json
 import os
@@ -92,10 +96,46 @@ def _add_lora(model, ft_config):
 def _pick_reader(ft_config, tokenizer):
     from . import train_data
     readers = {"txt": train_data.TrainTxt, "alpaca": train_data.TrainSAD, "gpt4all": train_data.TrainGPT4All,
-               "bluemoon": train_data.TrainBlueMoon}
+               "bluemoon": train_data.TrainBlueMoon, "preference": train_data.TrainPreference}
     if ft_config.ds_type not in readers:
         raise NotImplementedError("ERROR: Unknown dataset format")
     return readers[ft_config.ds_type](ft_config.dataset, ft_config.val_set_size, tokenizer, ft_config.cutoff_len)
+
+
+def _preference_trainer():
+    """transformers.Trainer with the loss of pairs: batches as train_data.collate_pairs makes them."""
+    import transformers
+    from . import preference
+
+    class PreferenceTrainer(transformers.Trainer):
+        def __init__(self, *args, beta=0.1, label_smoothing=0.0, **kwargs):
+            super().__init__(*args, **kwargs)
+            self.beta, self.label_smoothing = beta, label_smoothing
+            self.model_accepts_loss_kwargs = False       # the loss is a mean over pairs: micro-batches are averaged, not weighted by their tokens
+            self._margins = {True: [], False: []}
+
+        def compute_loss(self, model, inputs, return_outputs=False, num_items_in_batch=None):
+            labels = preference.shifted_labels(inputs["labels"])
+            rows = {k: inputs[k] for k in ("input_ids", "attention_mask")}
+            plain = self.accelerator.unwrap_model(model)
+            with torch.no_grad(), preference.adapters_off(plain):
+                ref = preference.token_logps(plain(**rows, use_cache=False).logits, labels)
+            logits = model(**rows, use_cache=False).logits
+            loss, rewards = preference.preference_loss(logits, labels, ref, self.beta, self.label_smoothing)
+            pairs = rewards.numel() // 2
+            self._margins[model.training].append(rewards[:pairs] - rewards[pairs:])
+            return (loss, {"rewards": rewards}) if return_outputs else loss
+
+        def log(self, logs, *args, **kwargs):
+            """With every line of losses the share of pairs that are the right way round, and by how much."""
+            for training, key, prefix in ((True, "loss", ""), (False, "eval_loss", "eval_")):
+                if key in logs and self._margins[training]:
+                    margins = torch.cat(self._margins[training])
+                    self._margins[training] = []
+                    logs = {**logs, prefix + "accuracy": round(float((margins > 0).float().mean()), 4), prefix + "margin": round(float(margins.mean()), 6)}
+            return super().log(logs, *args, **kwargs)
+
+    return PreferenceTrainer
 
 
 def _train(model, tokenizer, data, ft_config):
@@ -128,10 +168,17 @@ def _train(model, tokenizer, data, ft_config):
         load_best_model_at_end=False,
         ddp_find_unused_parameters=False if ft_config.ddp else None,
         report_to="none",
+        remove_unused_columns=ft_config.ds_type != "preference",
+        prediction_loss_only=ft_config.ds_type == "preference",
     )
-    trainer = transformers.Trainer(
-        model=model, train_dataset=data.train_data, eval_dataset=data.val_data if eval_steps else None, args=args,
-        data_collator=transformers.DataCollatorForLanguageModeling(tokenizer, mlm=False))
+    datasets = dict(train_dataset=data.train_data, eval_dataset=data.val_data if eval_steps else None)
+    if ft_config.ds_type == "preference":
+        from .train_data import collate_pairs
+        trainer = _preference_trainer()(model=model, args=args, **datasets, data_collator=lambda samples: collate_pairs(samples, tokenizer.pad_token_id),
+                                        beta=ft_config.beta, label_smoothing=ft_config.label_smoothing)
+    else:
+        trainer = transformers.Trainer(model=model, args=args, **datasets,
+                                       data_collator=transformers.DataCollatorForLanguageModeling(tokenizer, mlm=False))
     model.config.use_cache = False
     if ft_config.verbose:
         transformers.logging.set_verbosity_info()
@@ -195,7 +242,13 @@ def main(argv=None):
         if ft_config.gradient_checkpointing:
             print("Applying gradient checkpointing ...")
             from .gradient_checkpointing import apply_gradient_checkpointing
-            apply_gradient_checkpointing(model, checkpoint_ratio=ft_config.gradient_checkpointing_ratio)
+            apply_gradient_checkpointing(model, checkpoint_ratio=ft_config.gradient_checkpointing_ratio, bits=ft_config.act_bits)
+        if ft_config.act_bits == 8:
+            if ft_config.v1:
+                print("note: v1 layers are not fused; their MLP blocks keep their activations as they are")
+            else:
+                from .model_attn_mlp_patch import make_fused_mlp
+                print(make_fused_mlp(model, act_bits=8), "MLP blocks keep their activations in 8 bits")
         if not ft_config.ddp and torch.cuda.device_count() > 1:
             model.is_parallelizable = True           # keeps Trainer from wrapping the model in DataParallel
             model.model_parallel = True

@@ -24,6 +24,7 @@ import threading
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import autograd_4bit, matmul_utils_4bit
 from .autograd_4bit import Autograd4bitQuantLinear, _buffer, _has_bias, _weight, fuse_quant_linears
@@ -389,6 +390,7 @@ def ungroup(model):
             del m.__dict__['forward']
             m.__dict__.pop('_q4_mlp_args', None)
             m.__dict__.pop('_q4_mlp_gated', None)
+            m.__dict__.pop('_q4_act_bits', None)
     return count
 
 
@@ -517,6 +519,24 @@ class _SiluMul(torch.autograd.Function):
         return quant_hip.silu_mul_bwd(dout, gate, up)
 
 
+class _SiluMulAct8(torch.autograd.Function):
+    """silu(gate) * up that keeps gate and up in 8 bits: 17 bits an element of the block for its backward pass in place of 32.  The output is that of the
+    operands as they are (formed in fp32, one rounding), the gradients those at the values held."""
+
+    @staticmethod
+    def forward(ctx, gate, up):
+        from . import quant_hip
+        out, kept = quant_hip.silu_mul_act8(gate, up)
+        ctx.save_for_backward(*kept)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        from . import quant_hip
+        return quant_hip.silu_mul_act8_bwd(dout, ctx.saved_tensors)
+
+
 def _gated_rows_forward(mlp, x):
     """The block's forward above the decode sizes: its own three layers, silu(gate) * up in one pass (us, forward / backward, 1024 x
     11008: 24 / 37 as five elementwise kernels, 16 / 24 as two).  Only for forwards known to be this expression."""
@@ -524,7 +544,9 @@ def _gated_rows_forward(mlp, x):
     gate, up = mlp.gate_proj(x), mlp.up_proj(x)
     if not quant_hip.silu_mul_takes(gate, up):
         return mlp.down_proj(mlp.act_fn(gate) * up)
-    return mlp.down_proj(_SiluMul.apply(gate, up) if torch.is_grad_enabled() else quant_hip.silu_mul(gate, up))
+    if not torch.is_grad_enabled():
+        return mlp.down_proj(quant_hip.silu_mul(gate, up))
+    return mlp.down_proj((_SiluMulAct8 if mlp.__dict__.get('_q4_act_bits') == 8 else _SiluMul).apply(gate, up))
 
 
 def _act_unobserved(mlp):
@@ -590,13 +612,19 @@ def _mlp_decode_forward(mlp, x):
     return d['_q4_mlp_forward'](x)
 
 
-def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step=True):
+def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step=True, act_bits=16):
     """One launch for gate_proj / up_proj of every MLP block (model_attn_mlp_patch.py:163-247; the reference's Triton
     fused-MLP kernel is replaced by one launch over both projections followed by the block's own activation).  In place
     by default; then, with `fuse_decode_step` and a SiLU block of three 4-bit layers of the same group size, the block's
-    forward runs the whole decode step (gate, up, silu(gate) * up, down) as one launch or two."""
+    forward runs the whole decode step (gate, up, silu(gate) * up, down) as one launch or two.  `act_bits=8`: such a block, trained,
+    keeps the outputs of gate and up for its backward pass in 8 bits where its forward is known to be that expression (in place and
+    `fuse_decode_step` only)."""
     if is_v1_model:
         raise NotImplementedError("v1 (fp zeros) layers are not fused")
+    if act_bits not in (8, 16):
+        raise ValueError(f"act_bits must be 8 or 16 (as they are), not {act_bits}")
+    if act_bits == 8 and (concatenate or not fuse_decode_step):
+        raise ValueError("act_bits=8 needs blocks that are fused in place, with fuse_decode_step")
     names = ("gate_proj", "up_proj")
     count = 0
     for m in list(model.modules()):
@@ -613,6 +641,8 @@ def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step
                     and down.out_features == m.gate_proj.in_features and '_q4_mlp_forward' not in m.__dict__):
                 import types
                 m.__dict__['_q4_mlp_gated'] = _is_gated_forward(m.forward)
+                if act_bits == 8 and m.__dict__['_q4_mlp_gated']:
+                    m.__dict__['_q4_act_bits'] = 8
                 m.__dict__['_q4_mlp_forward'] = m.forward                # the block's own (bound) forward
                 m.__dict__['forward'] = types.MethodType(_mlp_decode_forward, m)
     if concatenate and torch.cuda.is_available():

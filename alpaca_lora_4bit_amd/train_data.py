@@ -14,6 +14,8 @@ Sample construction follows the reference:
   input section to appear, empty or not.
 * GPT4All records (`:254-330`): prompt (at most half the window), newline, response without BOS, EOS when it fits;
   labels are -100 over prompt, newline and padding.
+* preference records (no counterpart in the reference): a prompt and two answers, "chosen" and "rejected"; each answer becomes a sample like a
+  GPT4All record's, unpadded, and `collate_pairs` puts the chosen ones of a batch before the rejected ones.
 """
 import os
 from abc import ABC, abstractmethod
@@ -203,3 +205,58 @@ class TrainGPT4All(ATrainData):
             records = parts["train"]
             self.val_data = encode(parts["test"])
         self.train_data = encode(records)
+
+
+class TrainPreference(ATrainData):
+    """Records of a prompt, the answer to prefer to it and the one to reject: "prompt" (or Alpaca's "instruction" and "input"), "chosen", "rejected"."""
+
+    def __init__(self, dataset: str, val_set_size, tokenizer, cutoff_len) -> None:
+        super().__init__(dataset, val_set_size, tokenizer, cutoff_len)
+
+    def tokenize(self, prompt: str, use_eos_token=True, **kwargs) -> Dict[str, Any]:
+        pass                                       # unused: rows are built by tokenize_pair
+
+    def _ids(self, text, room, first=False):
+        """Ids of `text`, at most `room`; without BOS unless it comes `first`."""
+        ids = list(self.tokenizer(text)["input_ids"])
+        if not first and ids and ids[0] == self.tokenizer.bos_token_id:
+            ids = ids[1:]
+        return ids[:max(room, 0)]
+
+    def tokenize_pair(self, record, use_eos_token=True):
+        tok, window = self.tokenizer, self.cutoff_len
+        if record.get("prompt") is not None:
+            prompt = record["prompt"]
+        else:                                      # the template of the Alpaca records, up to where the answer begins
+            prompt = TrainSAD.generate_prompt(self, {**{k: v for k, v in record.items() if k in ("instruction", "input") and v is not None}, "output": ""})
+        head = self._ids(prompt, window // 2, first=True)
+        head += self._ids("\n", window - len(head))
+        sample = {}
+        for name in ("chosen", "rejected"):
+            answer = self._ids(record[name], window - len(head))
+            if use_eos_token and len(head) + len(answer) < window:         # a truncated answer gets no EOS
+                answer = answer + [tok.eos_token_id]
+            sample[name + "_ids"] = head + answer
+            sample[name + "_labels"] = [-100] * len(head) + answer
+        return sample
+
+    def prepare_data(self, use_eos_token=True, **kwargs) -> None:
+        def encode(split):
+            return split.map(lambda record: self.tokenize_pair(record, use_eos_token=use_eos_token), remove_columns=split.column_names)
+
+        records = _load_json(self.dataset)["train"]
+        self.val_data = None
+        if self.val_set_size > 0:
+            parts = records.train_test_split(test_size=self.val_set_size, shuffle=True, seed=_SPLIT_SEED)
+            records = parts["train"]
+            self.val_data = encode(parts["test"])
+        self.train_data = encode(records)
+
+
+def collate_pairs(samples, pad_token_id):
+    """input_ids, attention_mask and labels [2P, longest] of P samples of `TrainPreference`: the chosen answers' rows, then the rejected ones'."""
+    rows = [(s[name + "_ids"], s[name + "_labels"]) for name in ("chosen", "rejected") for s in samples]
+    longest = max(len(ids) for ids, _ in rows)
+    return {"input_ids": torch.tensor([ids + [pad_token_id] * (longest - len(ids)) for ids, _ in rows]),
+            "attention_mask": torch.tensor([[1] * len(ids) + [0] * (longest - len(ids)) for ids, _ in rows]),
+            "labels": torch.tensor([labels + [-100] * (longest - len(labels)) for _, labels in rows])}
