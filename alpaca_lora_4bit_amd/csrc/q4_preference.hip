@@ -27,6 +27,12 @@ template <typename T>
 __device__ __forceinline__ Pack<T> load_pack(const T* p) { return __builtin_bit_cast(Pack<T>, *reinterpret_cast<const uint4_t*>(p)); }
 template <typename T>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T>& r) { *reinterpret_cast<uint4_t*>(p) = __builtin_bit_cast(uint4_t, r); }
+// past the caches: a gradient of long rows is more than they hold
+template <bool PAST, typename T>
+__device__ __forceinline__ void store_grad(T* p, const Pack<T>& r) {
+    if constexpr (PAST) __builtin_nontemporal_store(__builtin_bit_cast(uint4_t, r), reinterpret_cast<uint4_t*>(p));
+    else store_pack(p, r);
+}
 
 // Values before the first 16-byte boundary of a row, packs behind it, values left.
 template <typename T>
@@ -108,7 +114,7 @@ __device__ __forceinline__ double group_sum(double v, double* lds) {
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_logps_kernel(LogitsView a, const long long* __restrict__ labels, float* __restrict__ logps, double* __restrict__ wide,
                                                               float2* __restrict__ stats) {
-    constexpr int N = Pack<T>::N, WAVES = THREADS / 64, U = 4;
+    constexpr int N = Pack<T>::N, WAVES = THREADS / 64, U = THREADS == 256 ? 8 : 4;
     __shared__ float sm[WAVES];
     __shared__ double ss[WAVES];
     const int tid = threadIdx.x;
@@ -165,6 +171,7 @@ template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_logps_bwd_kernel(LogitsView a, const long long* __restrict__ labels, const float2* __restrict__ stats,
                                                                   const float* __restrict__ coef, int per, const float* __restrict__ factor, T* __restrict__ dx) {
     constexpr int N = Pack<T>::N, U = 4;
+    constexpr bool PAST = THREADS == 1024;
     const int tid = threadIdx.x;
     const long rows = (long)a.B * a.S;
     for (long row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -175,7 +182,7 @@ __global__ __launch_bounds__(THREADS) void token_logps_bwd_kernel(LogitsView a, 
             Pack<T> zero;
 #pragma unroll
             for (int e = 0; e < N; ++e) zero.v[e] = (T)0.f;
-            for (int i = tid; i < so.packs; i += THREADS) store_pack(out + so.head + (long)i * N, zero);
+            for (int i = tid; i < so.packs; i += THREADS) store_grad<PAST>(out + so.head + (long)i * N, zero);
             if (tid < so.head) out[tid] = (T)0.f;
             if (tid < so.tail) out[so.head + (long)so.packs * N + tid] = (T)0.f;
             continue;
@@ -207,7 +214,7 @@ __global__ __launch_bounds__(THREADS) void token_logps_bwd_kernel(LogitsView a, 
                         for (int e = 0; e < N; ++e)
                             if (label == at + e) g.v[e] = own(p[u].v[e]);
                     }
-                    store_pack(out + at, g);
+                    store_grad<PAST>(out + at, g);
                 }
             }
             if (tid < sp.head) out[tid] = tid == label ? own(x[tid]) : share(x[tid]);
@@ -301,8 +308,9 @@ int by_type(int type, F&& launch) {
 }  // namespace q4
 
 // Threads of a row's workgroup.  Wavefronts by themselves for rows of up to 4 KB (32768 rows of 640 bytes, forward / backward: 64 threads 15 / 17 us,
-// 256 34 / 39).  Forward 256, and 512 where there are few rows or long ones (37 rows of 64 KB: 7.6 against 8.5 us, 2048 of 256 KB 96 against 110; 1024 threads
-// wait for each other: 32768 rows of 64 KB 415 against 199).  Backward, where nothing waits, 1024 for rows of 48 KB and more (the same rows 587 against 626).
+// 256 34 / 39).  Forward 256 with eight loads a thread on their way (32768 rows of 64 KB, 0.55 of them tokens: 190 us, four loads 198), and 512 where there are few
+// rows or long ones (37 rows of 64 KB: 7.6 against 8.5, 2048 of 256 KB 96 against 110; 1024 threads wait for each other: 415 against 190).  Backward, where
+// nothing waits, 1024 for rows of 48 KB and more, its stores past the caches (the same rows: 520 us, through them 587, with 256 threads 622).
 namespace {
 template <typename F>
 void by_width(bool forward, long rows, long bytes, F&& launch) {
