@@ -1,8 +1,8 @@
 // Log-probabilities of the tokens of answers from logits, their gradient, and the loss of pairs of answers (paired log ratios).
 //
-//   logp = (x_l - m) - log(sum of exp(x - m)) for any m        dx = c (1[l] - exp(x - m - log sum))
+//   logp = x_l - L        L = m + log(sum of exp(x - m)) for any m        dx = c (1[l] - exp(x - L))
 //
-// HBM-bound: one pass over a row's logits, backward one pass more from the two numbers (m, log sum) that forward left.  Rows whose label is not one of the V words are no tokens of an answer (a prompt,
+// HBM-bound: one pass over a row's logits, backward one pass more from the L that forward left.  Rows whose label is not one of the V words are no tokens of an answer (a prompt,
 // padding): they are not read, and their gradient is zero.  Exponentials and a lane's sum in fp32, what follows in fp64: a log ratio is the small
 // difference of sums of some hundred log-probabilities, and an error in one direction grows with the answer.
 #include "q4_common.hpp"
@@ -162,7 +162,10 @@ __global__ __launch_bounds__(THREADS) void token_logps_kernel(LogitsView a, cons
             const double total = log(s + kExpShort * (s - 1.0)), lp = ((double)mine - (double)at) - total;
             if (logps) logps[row] = (float)lp;
             else wide[row] = lp;
-            stats[row] = float2{at, (float)total};
+            // what backward takes: L in two parts, so that logits near it lose nothing when it is taken off (a row of the lowest number has all of
+            // the sum's logarithm in the second)
+            const float most = (float)((double)at + total);
+            stats[row] = float2{most, (float)(total - ((double)most - (double)at))};
         }
     }
 }

@@ -527,14 +527,14 @@ class _SiluMulAct8(torch.autograd.Function):
     def forward(ctx, gate, up):
         from . import quant_hip
         out, kept = quant_hip.silu_mul_act8(gate, up)
-        ctx.save_for_backward(*kept)
+        ctx.save_for_backward(kept)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         from . import quant_hip
-        return quant_hip.silu_mul_act8_bwd(dout, ctx.saved_tensors)
+        return quant_hip.silu_mul_act8_bwd(dout, ctx.saved_tensors[0])
 
 
 def _gated_rows_forward(mlp, x):

@@ -35,8 +35,9 @@ def preference_loss(logits, labels, ref_logps, beta=0.1, label_smoothing=0.0):
 
 @contextlib.contextmanager
 def adapters_off(model):
-    """Within it the model computes without its LoRA adapters; each layer gets its own state back afterwards."""
-    layers = [(m, m.disable_adapters) for m in model.modules() if "Linear4bitLt" in str(type(m))]
+    """Within it the model computes without its LoRA adapters (Linear4bitLt's, and those of peft's own layers beside them); each layer gets its own
+    state back afterwards."""
+    layers = [(m, m.disable_adapters) for m in model.modules() if hasattr(m, "lora_A") and hasattr(m, "enable_adapters")]
     try:
         for layer, _ in layers:
             layer.enable_adapters(False)

@@ -1098,13 +1098,13 @@ def act8_unpack(codes, scales, dtype=torch.float16):
 
 
 def silu_mul_act8(gate, up):
-    """(silu(gate) * up, kept) for gate, up fp16 or bf16 of one shape; the product is formed in fp32 and rounded once, and kept = (gate's codes, gate's
-    scales, up's codes, up's scales) as act8_pack gives them."""
+    """(silu(gate) * up, kept) for gate, up fp16 or bf16 of one shape; the product is formed in fp32 and rounded once.  `kept` (uint8, 17 bits for each
+    element of gate) holds both as act8_pack does: gate's codes, up's codes, gate's scales, up's scales, each from a multiple of 16 bytes on."""
     return _training().silu_mul_act8(gate, up)
 
 
 def silu_mul_act8_bwd(dout, kept):
-    """(dgate, dup) of silu(gate) * up in dout's type (fp16 or bf16), at the values that `kept` holds."""
+    """(dgate, dup) of silu(gate) * up in dout's type (fp16 or bf16) and shape, at the values that `kept` holds."""
     return _training().silu_mul_act8_bwd(dout, kept)
 
 

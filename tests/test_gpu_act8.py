@@ -24,6 +24,17 @@ def _check(x, codes, scales, oracle8):
     assert np.array_equal(_np(scales), s, equal_nan=True)
 
 
+def _parts(kept, x):
+    """(codes, scales, codes, scales) of gate and up in what a gated activation keeps for tensors like x."""
+    import torch
+    n, blocks = x.numel(), -(-x.numel() // 32)
+    c, s = -(-n // 16) * 16, -(-2 * blocks // 16) * 16
+    assert kept.dtype == torch.uint8 and kept.shape == (2 * (c + s),)
+    codes = [kept[i * c:i * c + n].view(torch.int8).view(x.shape) for i in (0, 1)]
+    scales = [kept[2 * c + i * s:2 * c + i * s + 2 * blocks].view(torch.bfloat16) for i in (0, 1)]
+    return codes[0], scales[0], codes[1], scales[1]
+
+
 @pytest.fixture(scope="module")
 def oracle8():
     from oracle import training_oracle
@@ -105,8 +116,9 @@ def test_inputs_that_lie_otherwise(view, oracle8):
     _check(x, codes, scales, oracle8)
     out, kept = qh.silu_mul_act8(x, x)
     again, kept2 = qh.silu_mul_act8(x.clone(memory_format=torch.contiguous_format), x.contiguous())
-    assert torch.equal(out, again) and all(torch.equal(a, b) for a, b in zip(kept, kept2))
-    assert torch.equal(kept[0], codes) and torch.equal(kept[3], scales)
+    parts = _parts(kept, x)
+    assert torch.equal(out, again) and all(torch.equal(a, b) for a, b in zip(parts, _parts(kept2, x)))
+    assert torch.equal(parts[0], codes) and torch.equal(parts[3], scales)
     for a, b in zip(qh.silu_mul_act8_bwd(x, kept), qh.silu_mul_act8_bwd(x.contiguous(), kept)):
         assert torch.equal(a, b)
 
@@ -123,8 +135,9 @@ def test_gated_activation(kind, shape, oracle8):
     gate, up, dout = gate.to(dt), up.to(dt), dout.to(dt)
     u, tiny = torch.finfo(dt).eps / 2, TINY[kind]
     out, kept = qh.silu_mul_act8(gate, up)
-    _check(gate, kept[0], kept[1], oracle8)
-    _check(up, kept[2], kept[3], oracle8)
+    parts = _parts(kept, gate)
+    _check(gate, *parts[:2], oracle8)
+    _check(up, *parts[2:], oracle8)
     want = oracle8.silu_mul(_np(gate), _np(up))
     assert (np.abs(_np(out) - want) <= (u + 2.0 ** -15) * np.abs(want) + tiny + 2.0 ** -126 * np.abs(_np(gate) * _np(up))).all()
     dgate, dup = qh.silu_mul_act8_bwd(dout, kept)
@@ -170,7 +183,8 @@ def test_refused_and_empty_calls():
                 lambda: qh.act8_unpack(codes.view(-1)[1:1000], scales[:32]), lambda: qh.act8_unpack(codes, scales.cpu()),
                 lambda: qh.silu_mul_act8(x, x.bfloat16()), lambda: qh.silu_mul_act8(x.float(), x.float()), lambda: qh.silu_mul_act8(x, x[:20]),
                 lambda: qh.silu_mul_act8(x, x.cpu()), lambda: qh.silu_mul_act8_bwd(out[:20], kept), lambda: qh.silu_mul_act8_bwd(out.float(), kept),
-                lambda: qh.silu_mul_act8_bwd(out, (kept[0], kept[1][:-1], kept[2], kept[3])), lambda: qh.silu_mul_act8_bwd(out.cpu(), kept)):
+                lambda: qh.silu_mul_act8_bwd(out, kept[:-16]), lambda: qh.silu_mul_act8_bwd(out, kept.view(torch.int8)), lambda: qh.silu_mul_act8_bwd(out, kept.cpu()),
+                lambda: qh.silu_mul_act8_bwd(out.cpu(), kept)):
         with pytest.raises(ValueError):
             bad()
     with torch.autograd.forward_ad.dual_level():
