@@ -996,18 +996,23 @@ struct Kept {
     }
 };
 
-std::pair<at::Tensor, at::Tensor> silu_mul_act8(const at::Tensor& gate, const at::Tensor& up) {
+std::pair<at::Tensor, c10::optional<at::Tensor>> silu_mul_act8(const at::Tensor& gate, const at::Tensor& up, bool keep) {
     check_count(gate, "gate");
     check_count(up, "up");
     const int type = type_of(gate, false, "gate");
     TORCH_CHECK_VALUE(up.scalar_type() == gate.scalar_type() && up.sizes() == gate.sizes() && up.device() == gate.device(), "up must be like gate");
     const at::Tensor g = in_one_piece(gate), u = in_one_piece(up);
     const int64_t n = gate.numel();
-    at::Tensor out = at::empty(gate.sizes(), gate.options()), kept = at::empty({Kept::bytes(n)}, gate.options().dtype(at::kByte));
+    at::Tensor out = at::empty(gate.sizes(), gate.options());
+    c10::optional<at::Tensor> kept;
+    c10::optional<Kept> k;
+    if (keep) {
+        kept = at::empty({Kept::bytes(n)}, gate.options().dtype(at::kByte));
+        k.emplace(*kept, n);
+    }
     if (n == 0) return {out, kept};
-    const Kept k(kept, n);
     Launch L(gate.device());
-    const int rc = q4_silu_mul_act8(g.data_ptr(), u.data_ptr(), type, out.data_ptr(), &k.gate, &k.up, n, L.stream);
+    const int rc = q4_silu_mul_act8(g.data_ptr(), u.data_ptr(), type, out.data_ptr(), keep ? &k->gate : nullptr, keep ? &k->up : nullptr, n, L.stream);
     if (rc != Q4_OK) raise_q4(rc, "q4_silu_mul_act8");
     return {out, kept};
 }
@@ -1215,7 +1220,7 @@ PYBIND11_MODULE(_q4_host, m) {
     m.def("lora_rows", &lora_rows, py::arg("x"), py::arg("index"), py::arg("specs"), py::arg("per") = 1);
     m.def("act8_pack", &act8_pack, py::arg("x"));
     m.def("act8_unpack", &act8_unpack, py::arg("codes"), py::arg("scales"), py::arg("dtype"));
-    m.def("silu_mul_act8", &silu_mul_act8, py::arg("gate"), py::arg("up"));
+    m.def("silu_mul_act8", &silu_mul_act8, py::arg("gate"), py::arg("up"), py::arg("keep") = true);
     m.def("silu_mul_act8_bwd", &silu_mul_act8_bwd, py::arg("dout"), py::arg("kept"));
     m.def("token_logps", &token_logps, py::arg("logits"), py::arg("labels"));
     m.def("token_logps_bwd", &token_logps_bwd, py::arg("logits"), py::arg("labels"), py::arg("stats"), py::arg("coef"), py::arg("factor") = py::none());

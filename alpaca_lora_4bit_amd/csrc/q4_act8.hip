@@ -127,11 +127,10 @@ __global__ __launch_bounds__(kAct8Threads) void act8_unpack_kernel(const int8_t*
 // 1 / (1 + exp(-x)); zero where it would be less than the least normal fp32, below -87
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 
-// out = silu(gate) * up from the operands as they are, in fp32 and rounded once; both operands kept in 8 bits.
-template <typename T>
-__global__ __launch_bounds__(kAct8Threads) void silu_mul_act8_kernel(const T* __restrict__ gate, const T* __restrict__ up, T* __restrict__ out,
-                                                                     int8_t* __restrict__ gate_codes, uint16_t* __restrict__ gate_scales,
-                                                                     int8_t* __restrict__ up_codes, uint16_t* __restrict__ up_scales, long n) {
+// out = silu(gate) * up from the operands as they are, in fp32 and rounded once; KEEP: both operands kept in 8 bits.
+template <typename T, bool KEEP>
+__global__ __launch_bounds__(kAct8Threads) void silu_mul_act8_kernel(const T* __restrict__ gate, const T* __restrict__ up, T* __restrict__ out, q4_act8_t kg, q4_act8_t ku,
+                                                                     long n) {
     const long c = (long)blockIdx.x * kAct8Threads + threadIdx.x;
     if (c >= act8_blocks(n) * 4) return;
     const Act8Eight<T> g = load_eight(gate, 8 * c, n), u = load_eight(up, 8 * c, n);
@@ -142,13 +141,15 @@ __global__ __launch_bounds__(kAct8Threads) void silu_mul_act8_kernel(const T* __
         o.v[e] = (T)(x * sigmoid(x) * (float)u.v[e]);
     }
     store_eight(out, 8 * c, n, o);
-    uint32_t gs, us;
-    const uint2_t gw = encode(g, &gs), uw = encode(u, &us);
-    store_codes(gate_codes, 8 * c, n, gw);
-    store_codes(up_codes, 8 * c, n, uw);
-    if (c % 4 == 0) {
-        gate_scales[c / 4] = (uint16_t)(gs >> 16);
-        up_scales[c / 4] = (uint16_t)(us >> 16);
+    if constexpr (KEEP) {
+        uint32_t gs, us;
+        const uint2_t gw = encode(g, &gs), uw = encode(u, &us);
+        store_codes((int8_t*)kg.codes, 8 * c, n, gw);
+        store_codes((int8_t*)ku.codes, 8 * c, n, uw);
+        if (c % 4 == 0) {
+            ((uint16_t*)kg.scales)[c / 4] = (uint16_t)(gs >> 16);
+            ((uint16_t*)ku.scales)[c / 4] = (uint16_t)(us >> 16);
+        }
     }
 }
 
@@ -211,8 +212,8 @@ int q4_launch_silu_mul_act8(const void* gate, const void* up, int type, void* ou
     using namespace q4;
     return by_type16(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(silu_mul_act8_kernel<T>, act8_grid(n), dim3(kAct8Threads), 0, stream, (const T*)gate, (const T*)up, (T*)out, (int8_t*)g->codes,
-                           (uint16_t*)g->scales, (int8_t*)u->codes, (uint16_t*)u->scales, n);
+        if (g) hipLaunchKernelGGL((silu_mul_act8_kernel<T, true>), act8_grid(n), dim3(kAct8Threads), 0, stream, (const T*)gate, (const T*)up, (T*)out, *g, *u, n);
+        else hipLaunchKernelGGL((silu_mul_act8_kernel<T, false>), act8_grid(n), dim3(kAct8Threads), 0, stream, (const T*)gate, (const T*)up, (T*)out, q4_act8_t{}, q4_act8_t{}, n);
     });
 }
 

@@ -49,6 +49,7 @@ extern "C" int q4_silu_mul_act8(const void* gate, const void* up, int type, void
     if (!gate || !up || !out) return Q4_ERR_NULL_POINTER;
     if ((type != Q4_TYPE_F16 && type != Q4_TYPE_BF16) || !fits(n)) return Q4_ERR_BAD_SHAPE;
     if (misaligned(gate) || misaligned(up) || misaligned(out)) return Q4_ERR_MISALIGNED;
+    if (!kept_gate && !kept_up) return q4_launch_silu_mul_act8(gate, up, type, out, nullptr, nullptr, (long)n, (hipStream_t)stream);
     int rc = check_kept(kept_gate);
     if (rc == Q4_OK) rc = check_kept(kept_up);
     return rc != Q4_OK ? rc : q4_launch_silu_mul_act8(gate, up, type, out, kept_gate, kept_up, (long)n, (hipStream_t)stream);

@@ -544,9 +544,11 @@ def _gated_rows_forward(mlp, x):
     gate, up = mlp.gate_proj(x), mlp.up_proj(x)
     if not quant_hip.silu_mul_takes(gate, up):
         return mlp.down_proj(mlp.act_fn(gate) * up)
-    if not torch.is_grad_enabled():
-        return mlp.down_proj(quant_hip.silu_mul(gate, up))
-    return mlp.down_proj((_SiluMulAct8 if mlp.__dict__.get('_q4_act_bits') == 8 else _SiluMul).apply(gate, up))
+    if mlp.__dict__.get('_q4_act_bits') == 8:                # the same product with and without gradients: a checkpointed block runs both ways
+        if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
+            return mlp.down_proj(_SiluMulAct8.apply(gate, up))
+        return mlp.down_proj(quant_hip.silu_mul_act8(gate, up, keep=False)[0])
+    return mlp.down_proj(_SiluMul.apply(gate, up) if torch.is_grad_enabled() else quant_hip.silu_mul(gate, up))
 
 
 def _act_unobserved(mlp):
@@ -631,6 +633,10 @@ def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step
         if all(hasattr(m, n) for n in names + ("down_proj",)):
             if concatenate:
                 count += bool(_fuse_children(m, names, "gate_up_proj"))
+                continue
+            if act_bits == 8 and m.__dict__.get('_q4_mlp_gated') and m.__dict__.get('_q4_act_bits') != 8:
+                m.__dict__['_q4_act_bits'] = 8                           # a block that an earlier call has fused
+                count += 1
                 continue
             group = _group_children(m, names)
             count += group is not None

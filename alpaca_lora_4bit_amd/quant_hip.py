@@ -1097,10 +1097,11 @@ def act8_unpack(codes, scales, dtype=torch.float16):
     return _training().act8_unpack(codes, scales, dtype)
 
 
-def silu_mul_act8(gate, up):
+def silu_mul_act8(gate, up, keep=True):
     """(silu(gate) * up, kept) for gate, up fp16 or bf16 of one shape; the product is formed in fp32 and rounded once.  `kept` (uint8, 17 bits for each
-    element of gate) holds both as act8_pack does: gate's codes, up's codes, gate's scales, up's scales, each from a multiple of 16 bytes on."""
-    return _training().silu_mul_act8(gate, up)
+    element of gate) holds both as act8_pack does: gate's codes, up's codes, gate's scales, up's scales, each from a multiple of 16 bytes on.
+    `keep=False`: the same product, and None."""
+    return _training().silu_mul_act8(gate, up, bool(keep))
 
 
 def silu_mul_act8_bwd(dout, kept):

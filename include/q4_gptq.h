@@ -436,7 +436,8 @@ Q4_API int q4_act8_pack(const void *x, int type, void *codes, void *scales, long
 /* x = code * scale, rounded to `type` (which need not be the packed one) and no further out than its largest number. */
 Q4_API int q4_act8_unpack(const void *codes, const void *scales, void *x, int type, long long n, void *stream);
 
-/* out = silu(gate) * up (model_attn_mlp_patch.py:224-228) from fp16 or bfloat16 gate, up [n], formed in fp32 and rounded once; both are kept in 8 bits.
+/* out = silu(gate) * up (model_attn_mlp_patch.py:224-228) from fp16 or bfloat16 gate, up [n], formed in fp32 and rounded once; both are kept in 8 bits
+ * (kept_gate and kept_up both NULL: the same product, nothing is kept).
  * Backward from what was kept: dup = dout * gate * s, dgate = dout * up * s * (1 + gate * (1 - s)) with s = sigmoid(gate).  n and alignment as above. */
 Q4_API int q4_silu_mul_act8(const void *gate, const void *up, int type, void *out, const q4_act8_t *kept_gate, const q4_act8_t *kept_up, long long n, void *stream);
 Q4_API int q4_silu_mul_act8_bwd(const void *dout, int type, const q4_act8_t *kept_gate, const q4_act8_t *kept_up, void *dgate, void *dup, long long n, void *stream);

@@ -235,3 +235,49 @@ def test_on_another_stream_and_in_captured_graphs():
         got = [o.clone() for o in step(*sets[0][0])]
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+
+
+def test_more_than_2_to_the_31_values(oracle8):
+    """The places of the last values pass 32 bits: what lies there comes out as it does by itself."""
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip as qh
+    n, tail = 2 ** 31 + 4096 + 37, 32 * 300 + 37
+    x = torch.zeros(n, dtype=torch.float16, device="cuda")
+    x[-tail:] = torch.randn(tail, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).half()
+    codes, scales = qh.act8_pack(x)
+    want = qh.act8_pack(x[-tail:].clone())
+    assert torch.equal(codes[-tail:], want[0]) and torch.equal(scales[-len(want[1]):], want[1]) and not bool(codes[:1000].any())
+    y = qh.act8_unpack(codes, scales)
+    assert torch.equal(y[-tail:], qh.act8_unpack(*want)) and not bool(y[:1000].any())
+    del codes, scales, y
+    out, kept = qh.silu_mul_act8(x, x)
+    dgate, dup = qh.silu_mul_act8_bwd(x, kept)
+    alone, kept_alone = qh.silu_mul_act8(x[-tail:].clone(), x[-tail:].clone())
+    a, b = qh.silu_mul_act8_bwd(x[-tail:].clone(), kept_alone)
+    assert torch.equal(out[-tail:], alone) and torch.equal(dgate[-tail:], a) and torch.equal(dup[-tail:], b) and not bool(dup[:1000].any())
+
+
+def test_the_product_alone():
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip as qh
+    for dt in (torch.float16, torch.bfloat16):
+        g, u = (torch.randn(7, 333, device="cuda").to(dt) for _ in range(2))
+        out, kept = qh.silu_mul_act8(g, u, keep=False)
+        assert kept is None and torch.equal(out, qh.silu_mul_act8(g, u)[0])
+
+
+def test_two_streams_at_once():
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip as qh
+    xs = [torch.randn(513, 4099, device="cuda").half() for _ in range(2)]
+    want = [(qh.act8_pack(x)[0], qh.silu_mul_act8(x, x)[0]) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, (x, s) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(s):
+                got[k].append((qh.act8_pack(x)[0], qh.silu_mul_act8(x, x)[0]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(a, b) for pair in got[k] for a, b in zip(pair, want[k]))

@@ -325,3 +325,48 @@ def test_a_captured_training_step():
         eager = step(w.detach().clone().requires_grad_())
         torch.cuda.synchronize()
         assert torch.equal(loss, eager[0]) and torch.equal(grad, eager[1])
+
+
+def test_more_than_2_to_the_31_logits(orc):
+    """Rows whose places pass 32 bits come out as they do by themselves, forward and backward, in log-probabilities and loss."""
+    import torch
+    from alpaca_lora_4bit_amd import preference, quant_hip as qh
+    v = 2 ** 20 + 3
+    x = torch.zeros((2, 1030, v), dtype=torch.float16, device="cuda")
+    labels = torch.full((2, 1030), -100, device="cuda")
+    x[:, -3:] = _logits((2, 3, v), "float16", 1)
+    labels[:, -3:] = torch.tensor([[5, v - 1, v // 2], [7, 0, 9]], device="cuda")
+    alone, mine = x[:, -3:].clone(), labels[:, -3:].clone()
+    lp, stats = qh.token_logps(x, labels)
+    want, _ = orc.token_logps(_np(alone), mine.cpu().numpy())
+    assert (np.abs(_np(lp[:, -3:]) - want) <= _logp_bound(want)).all() and not bool(lp[:, :-3].any())
+    ref = torch.full((2, 1030), -14.0, device="cuda")
+    loss, rewards, coef, stats = qh.preference_loss(x, labels, ref, 0.1)
+    loss2, rewards2, coef2, stats2 = qh.preference_loss(alone, mine, ref[:, :3], 0.1)
+    assert abs(float(loss - loss2)) < 1e-6 and bool(((rewards - rewards2).abs() < 1e-5).all())
+    scale = torch.tensor(4096.0, device="cuda")
+    dx = qh.token_logps_bwd(x, labels, stats, coef, scale)
+    dx2 = qh.token_logps_bwd(alone, mine, stats2, coef2, scale)
+    # rows that start elsewhere in a 16-byte piece add up in another order; the gradients are one rounding of what agrees to 2^-20
+    assert bool(((dx[:, -3:] - dx2).abs().float() <= 2.0 ** -10 * dx2.abs().float() + 2.0 ** -24).all()) and not bool(dx[0, 0].any()) and not bool(dx[1, 1026].any())
+
+
+def test_two_streams_at_once():
+    import torch
+    from alpaca_lora_4bit_amd import quant_hip as qh
+    sets = [(_logits((6, 70, 2003), "float16", k), _labels((6, 70), 2003, k), _logits((6, 70), "float32", k) - 6) for k in range(2)]
+
+    def step(x, labels, ref):
+        loss, rewards, coef, stats = qh.preference_loss(x, labels, ref, 0.1)
+        return loss, rewards, qh.token_logps_bwd(x, labels, stats, coef, loss)
+    want = [step(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(step(*sets[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(a, b) for outs in got[k] for a, b in zip(outs, want[k]))

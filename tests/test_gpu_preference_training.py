@@ -18,9 +18,9 @@ def _counted(monkeypatch, name):
     from alpaca_lora_4bit_amd import quant_hip
     seen, real = [], getattr(quant_hip, name)
 
-    def call(*a):
-        seen.append(tuple(a[0].shape))
-        return real(*a)
+    def call(*a, **kw):
+        seen.append(tuple(a[0].shape) if kw.get("keep", True) else None)
+        return real(*a, **kw)
     monkeypatch.setattr(quant_hip, name, call)
     return seen
 
@@ -146,10 +146,15 @@ def test_gated_block_that_keeps_8_bits(oracle, monkeypatch):
     assert want[2] - got[2] > 0.9 * M * I * (2 * 2 - 2 * 1.0625)      # at least gate and up of 16 bits less their 8 bits
     with torch.no_grad():
         calls.clear()
-        fused(xh)
-        assert not calls                                       # nothing is kept where nothing is differentiated
+        assert torch.equal(fused(xh), got[0]) and calls == [None]      # the same product, nothing kept where nothing is differentiated
+        calls.clear()
+    with torch.amp.autocast("cuda", dtype=torch.float16):
+        assert torch.equal(fused(xh), got[0]) and calls == [None]
+    calls.clear()
     ungroup(fused)
     assert "_q4_act_bits" not in fused.__dict__ and run(fused)[2] == want[2] and not calls
+    assert make_fused_mlp(fused) == 1 and run(fused)[0].shape == (M, H) and not calls
+    assert make_fused_mlp(fused, act_bits=8) == 1 and torch.equal(run(fused)[0], got[0]) and calls == [(M, I)]       # a block that is fused already
 
 
 def _model(tmp_path, oracle, seed=5):
@@ -228,5 +233,5 @@ def test_finetune_module_on_pairs(tmp_path, oracle, monkeypatch, chckpt, bits):
     assert all("accuracy" in h and "margin" in h for h in logs) and all("eval_accuracy" in h for h in evals)
     lora = [m for m in model.modules() if "Linear4bitLt" in str(type(m))]
     assert len(lora) == 4 and all(float(m.lora_B["default"].weight.detach().abs().max()) > 0 and not m.disable_adapters for m in lora)
-    assert bool(packs) == chckpt and bool(gated) == (bits == 8)
+    assert bool(packs) == chckpt and bool(gated) == (bits == 8) and (None in gated) == (bits == 8)
     assert len(load_file(os.path.join(out, "adapter_model.safetensors"))) == 8
