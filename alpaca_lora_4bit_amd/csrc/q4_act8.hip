@@ -81,7 +81,7 @@ __device__ __forceinline__ uint2_t encode(const Act8Eight<T>& r, uint32_t* scale
     *scale = sb;
     float s = __uint_as_float(sb);
     const bool some = s > 0.f;                                               // neither zero nor NaN
-    if constexpr (sizeof(T) == 4 || !__is_same(T, half_t)) {                 // fp16 has no values so small that 1 / s is out of range
+    if constexpr (!__is_same(T, half_t)) {                 // fp16 has no values so small that 1 / s is out of range
         const float lift = s < 0x1p-100f ? 0x1p64f : 1.f;
         s *= lift;
 #pragma unroll

@@ -25,8 +25,13 @@ struct Pack {
     static constexpr int N = 16 / sizeof(T);
     T v[N];
 };
+// a 16-byte load from any value's address
 template <typename T>
-__device__ __forceinline__ Pack<T> load_pack(const T* p) { return __builtin_bit_cast(Pack<T>, *reinterpret_cast<const uint4_t*>(p)); }
+__device__ __forceinline__ Pack<T> load_pack(const T* p) {
+    Pack<T> r;
+    __builtin_memcpy(&r, p, 16);
+    return r;
+}
 template <typename T>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T>& r) { *reinterpret_cast<uint4_t*>(p) = __builtin_bit_cast(uint4_t, r); }
 // past the caches: a gradient of long rows is more than they hold
@@ -36,7 +41,7 @@ __device__ __forceinline__ void store_grad(T* p, const Pack<T>& r) {
     else store_pack(p, r);
 }
 
-// Values before the first 16-byte boundary of a row, packs behind it, values left.
+// Values of a row before the first 16-byte boundary, packs behind it, values left.
 template <typename T>
 struct Split {
     int head, packs, tail;
@@ -133,22 +138,20 @@ __global__ __launch_bounds__(THREADS) void token_logps_kernel(LogitsView a, cons
         }
         const T* x = row_of<T>(a, row);
         const float mine = (float)x[label];
-        const Split<T> sp(x, a.V);
-        const T* body = x + sp.head;
+        const int packs = a.V / N, tail = a.V - packs * N;
         Sum r;
-        for (int i = tid; i < sp.packs; i += U * THREADS) {
+        for (int i = tid; i < packs; i += U * THREADS) {
             Pack<T> p[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {                                    // all on their way, the ones behind the end from the last place
                 const int k = i + u * THREADS;
-                p[u] = load_pack(body + (long)(k < sp.packs ? k : sp.packs - 1) * N);
+                p[u] = load_pack(x + (long)(k < packs ? k : packs - 1) * N);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (i + u * THREADS < sp.packs) r.add(p[u].v, mine);
+                if (i + u * THREADS < packs) r.add(p[u].v, mine);
         }
-        if (tid < sp.head) { const T one[1] = {x[tid]}; r.add(one, mine); }
-        if (tid < sp.tail) { const T one[1] = {body[(long)sp.packs * N + tid]}; r.add(one, mine); }
+        if (tid < tail) { const T one[1] = {x[(long)packs * N + tid]}; r.add(one, mine); }
         double s = group_sum<WAVES>((double)r.s - (double)r.lost, ss);
         float at = mine;
         if (!(s < 0x1p115)) {                                                // the same in all threads
@@ -182,8 +185,8 @@ __global__ __launch_bounds__(THREADS) void token_logps_bwd_kernel(LogitsView a, 
     for (long row = blockIdx.x; row < rows; row += gridDim.x) {
         const long long label = labels[row];
         T* out = dx + row * a.V;
+        const Split<T> so(out, a.V);                                         // stores from 16-byte boundaries on, loads from wherever that is
         if (label < 0 || label >= a.V) {
-            const Split<T> so(out, a.V);
             Pack<T> zero;
 #pragma unroll
             for (int e = 0; e < N; ++e) zero.v[e] = (T)0.f;
@@ -198,36 +201,31 @@ __global__ __launch_bounds__(THREADS) void token_logps_bwd_kernel(LogitsView a, 
         auto share = [&](T v) { return (T)(-c * __expf(((float)v - st.x) - st.y)); };
         // the label's own gradient c (1 - p), formed without that difference
         auto own = [&](T v) { return (T)(-c * expm1f(((float)v - st.x) - st.y)); };
-        const Split<T> sp(x, a.V);
-        if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0) {
-            for (int i = tid; i < sp.packs; i += U * THREADS) {
-                Pack<T> p[U];
+        for (int i = tid; i < so.packs; i += U * THREADS) {
+            Pack<T> p[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int k = i + u * THREADS;
-                    p[u] = load_pack(x + sp.head + (long)(k < sp.packs ? k : sp.packs - 1) * N);
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (i + u * THREADS >= sp.packs) break;
-                    const long at = sp.head + (long)(i + u * THREADS) * N;
-                    Pack<T> g;
-#pragma unroll
-                    for (int e = 0; e < N; ++e) g.v[e] = share(p[u].v[e]);
-                    if ((unsigned long)(label - at) < N) {
-#pragma unroll
-                        for (int e = 0; e < N; ++e)
-                            if (label == at + e) g.v[e] = own(p[u].v[e]);
-                    }
-                    store_grad<PAST>(out + at, g);
-                }
+            for (int u = 0; u < U; ++u) {
+                const int k = i + u * THREADS;
+                p[u] = load_pack(x + so.head + (long)(k < so.packs ? k : so.packs - 1) * N);
             }
-            if (tid < sp.head) out[tid] = tid == label ? own(x[tid]) : share(x[tid]);
-            const long at = sp.head + (long)sp.packs * N + tid;
-            if (tid < sp.tail) out[at] = at == label ? own(x[at]) : share(x[at]);
-        } else {                                                             // strides that put x and dx at different places of 16 bytes
-            for (long i = tid; i < a.V; i += THREADS) out[i] = i == label ? own(x[i]) : share(x[i]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i + u * THREADS >= so.packs) break;
+                const long at = so.head + (long)(i + u * THREADS) * N;
+                Pack<T> g;
+#pragma unroll
+                for (int e = 0; e < N; ++e) g.v[e] = share(p[u].v[e]);
+                if ((unsigned long)(label - at) < N) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (label == at + e) g.v[e] = own(p[u].v[e]);
+                }
+                store_grad<PAST>(out + at, g);
+            }
         }
+        if (tid < so.head) out[tid] = tid == label ? own(x[tid]) : share(x[tid]);
+        const long at = so.head + (long)so.packs * N + tid;
+        if (tid < so.tail) out[at] = at == label ? own(x[at]) : share(x[at]);
     }
 }
 

@@ -70,12 +70,11 @@ class NewForward(_ForwardPatch):
 
     def new_forward(self, *args, **kwargs):
         block = self._target
-        if not block.training:
+        if not block.training or not torch.is_grad_enabled():    # nothing to run again for
             return block.old_forward_for_cp(*args, **kwargs)
         hidden = args[0] if args else None
         # the graph holds a leaf (the embedding's output) in any case: 8 bits of it would be more memory, not less
-        packed = (self._bits == 8 and torch.is_grad_enabled() and torch.is_tensor(hidden) and hidden.requires_grad and not hidden.is_leaf
-                  and hidden.is_floating_point())
+        packed = self._bits == 8 and torch.is_tensor(hidden) and hidden.requires_grad and not hidden.is_leaf and hidden.is_floating_point()
         # keyword arguments (masks, position embeddings, caches) ride in the closure, as in the reference
         with _held_in_8_bits(hidden) if packed else contextlib.nullcontext():
             return checkpoint(lambda *inputs: block.old_forward_for_cp(*inputs, **kwargs), *args, use_reentrant=True)

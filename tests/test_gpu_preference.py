@@ -161,16 +161,15 @@ def test_logits_that_lie_otherwise(layout, orc):
     leaf = x.detach().clone(memory_format=torch.contiguous_format).requires_grad_()
     a = preference.token_logps(x, labels)
     b = preference.token_logps(leaf, labels)
+    assert torch.equal(a, b)                                   # where a row begins does not change the order of its sum
     view = x.detach().requires_grad_()
     assert view.stride() == x.stride()
     gout = torch.full_like(a, 0.25)
     (da,) = torch.autograd.grad(preference.token_logps(view, labels), view, gout)
     (db,) = torch.autograd.grad(b, leaf, gout.expand_as(a))
-    # rows that start elsewhere in a 16-byte piece add up in another order: half a step of fp16 either way, of values that agree to 2^-20
-    assert da.shape == x.shape and bool(((da - db).abs().float() <= 2.0 ** -10 * db.abs().float() + 2.0 ** -24).all())
+    assert da.shape == x.shape and torch.equal(da, db)
     want, soft = orc.token_logps(_np(x), labels.cpu().numpy())
-    for lp in (a, b):
-        assert (np.abs(_np(lp) - want) <= _logp_bound(want)).all()
+    assert (np.abs(_np(a) - want) <= _logp_bound(want)).all()
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -347,7 +346,7 @@ def test_more_than_2_to_the_31_logits(orc):
     scale = torch.tensor(4096.0, device="cuda")
     dx = qh.token_logps_bwd(x, labels, stats, coef, scale)
     dx2 = qh.token_logps_bwd(alone, mine, stats2, coef2, scale)
-    # rows that start elsewhere in a 16-byte piece add up in another order; the gradients are one rounding of what agrees to 2^-20
+    # few rows are added up by more threads, in another order; the gradients are one rounding of what agrees to 2^-20
     assert bool(((dx[:, -3:] - dx2).abs().float() <= 2.0 ** -10 * dx2.abs().float() + 2.0 ** -24).all()) and not bool(dx[0, 0].any()) and not bool(dx[1, 1026].any())
 
 
