@@ -929,7 +929,7 @@ void lora_rows(const at::Tensor& x, const at::Tensor& index, const std::vector<R
 }
 
 // ---- training on pairs of answers, and what a step keeps for its backward pass -------------------------------------------------
-// Tensors come from the caching allocator call by call, workspaces too.  The gradients are the Python layer's autograd functions'.
+// Tensors come from the caching allocator call by call, workspaces too, so that captured graphs share none.
 
 int type_of(const at::Tensor& t, bool wide, const char* what) {
     const auto s = t.scalar_type();
@@ -1053,7 +1053,7 @@ Answers check_answers(const at::Tensor& logits, const at::Tensor& labels) {
     at::Tensor x = logits;
     if (x.dim() < 3) x = x.unsqueeze(0);
     if (x.dim() < 3) x = x.unsqueeze(0);
-    if (x.dim() > 3) x = x.reshape({-1, x.size(-2), a.V});
+    if (x.dim() > 3) x = x.reshape({x.size(-2) ? labels.numel() / x.size(-2) : 0, x.size(-2), a.V});
     if (x.stride(2) != 1 && a.V > 1) x = x.contiguous();
     a.logits = x;
     a.B = x.size(0);

@@ -104,7 +104,8 @@ def checkpoint_locations(n_layers: int, checkpoint_ratio=1) -> np.ndarray:
 
 
 def apply_gradient_checkpointing(model, checkpoint_ratio=1, bits=16):
-    """Patches `model` in place; returns (list of NewForward, VarWrapper of the first embedding or None).  `bits=8`: the checkpoints in 8 bits."""
+    """Patches `model` in place; returns (list of NewForward, VarWrapper of the first embedding or None).  `bits=8`: the checkpoints in 8 bits
+    (hidden states in fp16, bf16 or fp32 on the GPU)."""
     layer_type = _decoder_layer_type()
     blocks = [m for _, m in model.named_modules() if isinstance(m, layer_type)]
     patched = []

@@ -620,7 +620,7 @@ def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step
     by default; then, with `fuse_decode_step` and a SiLU block of three 4-bit layers of the same group size, the block's
     forward runs the whole decode step (gate, up, silu(gate) * up, down) as one launch or two.  `act_bits=8`: such a block, trained,
     keeps the outputs of gate and up for its backward pass in 8 bits where its forward is known to be that expression (in place and
-    `fuse_decode_step` only)."""
+    `fuse_decode_step` only); second derivatives through it are refused."""
     if is_v1_model:
         raise NotImplementedError("v1 (fp zeros) layers are not fused")
     if act_bits not in (8, 16):

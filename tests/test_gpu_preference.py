@@ -250,6 +250,10 @@ def test_refused_calls():
         with pytest.raises(ValueError):
             bad()
     assert preference.token_logps(x[:0], labels[:0]).shape == (0, 5)
+    for shape in ((0, 2, 5, 40), (3, 2, 0, 40), (2, 0, 3, 40)):
+        e = torch.zeros(shape, device="cuda", requires_grad=True)
+        lp = preference.token_logps(e, torch.zeros(shape[:-1], device="cuda", dtype=torch.long))
+        assert lp.shape == shape[:-1] and torch.autograd.grad(lp.sum(), e)[0].shape == shape
     y = x.clone().requires_grad_()
     lp = preference.token_logps(y, labels)
     with pytest.raises(Exception):                             # a graph of the backward pass
