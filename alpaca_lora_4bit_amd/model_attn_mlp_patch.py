@@ -20,6 +20,8 @@ import math
 import os
 import re
 import threading
+import types
+import warnings
 
 import torch
 import torch.nn as nn
@@ -609,18 +611,48 @@ def _mlp_decode_forward(mlp, x):
                 faster = quant_hip.mlp_rows_is_faster(rows, args[4], args[5])
                 step = quant_hip.mlp_rows_prepared if faster or rows > mlp_decode_max_rows else quant_hip.mlp_decode_prepared
                 return step(x, args[0], args[1], args[2], args[3], tuple(x.shape[:-1]) + (args[6],))
+    return _mlp_gated_forward(mlp, x)
+
+
+def _mlp_gated_forward(mlp, x):
+    """The block's forward without the decode step, and all of it where the step does not take the block's layers."""
+    d = mlp.__dict__
     if x.is_cuda and d.get('_q4_mlp_gated') and _act_unobserved(mlp):
         return _gated_rows_forward(mlp, x)
     return d['_q4_mlp_forward'](x)
+
+
+def _route_mlp(mlp, forward):
+    """`forward` in the place of the block's own, which stays reachable."""
+    mlp.__dict__['_q4_mlp_gated'] = _is_gated_forward(mlp.forward)
+    mlp.__dict__['_q4_mlp_forward'] = mlp.forward            # the block's own (bound) forward
+    mlp.__dict__['forward'] = types.MethodType(forward, mlp)
+
+
+def _keep_8_bits(mlp):
+    """Marks a block that can keep gate and up in 8 bits, whatever the groups of its three 4-bit layers; whether it is one."""
+    layers = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
+    if not _is_silu(getattr(mlp, 'act_fn', None)) or not all(isinstance(l, Autograd4bitQuantLinear) and l.bits == 4 and not l.is_v1_model for l in layers):
+        return False
+    if '_q4_mlp_forward' not in mlp.__dict__:
+        if not _is_gated_forward(mlp.forward):
+            return False
+        _route_mlp(mlp, _mlp_gated_forward)
+    if not mlp.__dict__['_q4_mlp_gated']:
+        return False
+    mlp.__dict__['_q4_act_bits'] = 8
+    return True
 
 
 def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step=True, act_bits=16):
     """One launch for gate_proj / up_proj of every MLP block (model_attn_mlp_patch.py:163-247; the reference's Triton
     fused-MLP kernel is replaced by one launch over both projections followed by the block's own activation).  In place
     by default; then, with `fuse_decode_step` and a SiLU block of three 4-bit layers of the same group size, the block's
-    forward runs the whole decode step (gate, up, silu(gate) * up, down) as one launch or two.  `act_bits=8`: such a block, trained,
-    keeps the outputs of gate and up for its backward pass in 8 bits where its forward is known to be that expression (in place and
-    `fuse_decode_step` only); second derivatives through it are refused."""
+    forward runs the whole decode step (gate, up, silu(gate) * up, down) as one launch or two.  Returns the number of blocks grouped.
+
+    `act_bits=8` (in place and with `fuse_decode_step` only): SiLU blocks of three 4-bit layers, of any group sizes, whose forward is known to be that
+    expression keep the outputs of gate and up for their backward pass in 8 bits; second derivatives through them are refused.  Returns the number of blocks
+    that do; the others, which keep their operands as they are, are named in a warning."""
     if is_v1_model:
         raise NotImplementedError("v1 (fp zeros) layers are not fused")
     if act_bits not in (8, 16):
@@ -628,29 +660,29 @@ def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step
     if act_bits == 8 and (concatenate or not fuse_decode_step):
         raise ValueError("act_bits=8 needs blocks that are fused in place, with fuse_decode_step")
     names = ("gate_proj", "up_proj")
-    count = 0
-    for m in list(model.modules()):
+    count, as_they_are = 0, []
+    for path, m in list(model.named_modules()):
         if all(hasattr(m, n) for n in names + ("down_proj",)):
             if concatenate:
                 count += bool(_fuse_children(m, names, "gate_up_proj"))
                 continue
-            if act_bits == 8 and m.__dict__.get('_q4_mlp_gated') and m.__dict__.get('_q4_act_bits') != 8:
-                m.__dict__['_q4_act_bits'] = 8                           # a block that an earlier call has fused
-                count += 1
-                continue
             group = _group_children(m, names)
-            count += group is not None
             down = m.down_proj
             if (group is not None and fuse_decode_step and _is_silu(getattr(m, 'act_fn', None))
                     and isinstance(down, Autograd4bitQuantLinear) and down.bits == 4 and not down.is_v1_model
                     and down.groupsize == m.gate_proj.groupsize and down.in_features == m.gate_proj.out_features
                     and down.out_features == m.gate_proj.in_features and '_q4_mlp_forward' not in m.__dict__):
-                import types
-                m.__dict__['_q4_mlp_gated'] = _is_gated_forward(m.forward)
-                if act_bits == 8 and m.__dict__['_q4_mlp_gated']:
-                    m.__dict__['_q4_act_bits'] = 8
-                m.__dict__['_q4_mlp_forward'] = m.forward                # the block's own (bound) forward
-                m.__dict__['forward'] = types.MethodType(_mlp_decode_forward, m)
+                _route_mlp(m, _mlp_decode_forward)
+            if act_bits == 8:
+                kept = _keep_8_bits(m)
+                count += kept
+                if not kept:
+                    as_they_are.append(path or type(m).__name__)
+            else:
+                count += group is not None
+    if as_they_are:
+        warnings.warn(f"{len(as_they_are)} MLP blocks keep their activations as they are (not three 4-bit layers, another activation than SiLU, or a forward of "
+                      f"their own): {', '.join(as_they_are)}")
     if concatenate and torch.cuda.is_available():
         torch.cuda.empty_cache()
     return count

@@ -1,0 +1,77 @@
+"""MLP blocks that keep 8 bits, on the GPU: layers of any group sizes."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+H, I = 256, 512
+
+
+def _block(oracle, groupsize, seed=40):
+    import torch.nn as nn
+    from conftest import to_cuda_layer
+    from alpaca_lora_4bit_amd.autograd_4bit import Autograd4bitQuantLinear
+
+    class Gated(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.act_fn = nn.SiLU()
+
+        def forward(self, x):
+            return self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+    block = Gated()
+    for i, (name, k, n) in enumerate((("gate_proj", H, I), ("up_proj", H, I), ("down_proj", I, H))):
+        lin = Autograd4bitQuantLinear(k, n, groupsize=groupsize)
+        for key, v in to_cuda_layer(oracle.make_layer(k, n, lin.groupsize, seed=seed + i)).items():
+            if isinstance(v, torch.Tensor):
+                setattr(lin, key, v)
+        lin.bias = torch.zeros(n, dtype=torch.float16, device="cuda")
+        setattr(block, name, lin)
+    return block
+
+
+def _counted(monkeypatch, name):
+    from alpaca_lora_4bit_amd import quant_hip
+    seen, real = [], getattr(quant_hip, name)
+
+    def call(*a, **kw):
+        seen.append(tuple(a[0].shape) if kw.get("keep", True) else None)
+        return real(*a, **kw)
+    monkeypatch.setattr(quant_hip, name, call)
+    return seen
+
+
+def _x(oracle, rows, seed=4):
+    return torch.from_numpy(oracle.make_activations(rows, H, seed=seed)).cuda()
+
+
+@pytest.mark.parametrize("groupsize", [-1, 128])
+def test_a_block_keeps_8_bits_whatever_its_groups(oracle, monkeypatch, groupsize):
+    """Layers of one group a column too (gate's as wide as its input, down's as its own): outputs of the block's own forward to fp16's roundings, half as much kept."""
+    from conftest import rel_err
+    from alpaca_lora_4bit_amd.model_attn_mlp_patch import make_fused_mlp
+    rows = 640
+    own, marked = _block(oracle, groupsize), _block(oracle, groupsize)
+    assert make_fused_mlp(marked, act_bits=8) == 1
+    kept, backs = _counted(monkeypatch, "silu_mul_act8"), _counted(monkeypatch, "silu_mul_act8_bwd")
+    xh, dy = _x(oracle, rows), _x(oracle, rows, 5)
+
+    def run(block):
+        x = xh.clone().requires_grad_(True)
+        before = torch.cuda.memory_allocated()
+        with torch.amp.autocast("cuda", dtype=torch.float16):
+            y = block(x)
+        held = torch.cuda.memory_allocated() - before
+        y.backward(dy)
+        return y.detach(), x.grad, held
+    run(own), run(marked)                                      # allocations of the first calls
+    kept.clear(), backs.clear()
+    want, got = run(own), run(marked)
+    assert kept == backs == [(rows, I)]
+    # sums over 512 products of intermediates one fp16 rounding apart
+    assert rel_err(got[0].cpu().numpy(), want[0].double().cpu().numpy()) <= 3e-3
+    assert torch.isfinite(got[1]).all() and want[2] - got[2] > 0.9 * rows * I * (2 * 2 - 2 * 1.0625)
+    with torch.no_grad():
+        kept.clear()
+        assert marked(xh[:1]).shape == (1, H) and marked(xh[:12]).shape == (12, H)
+        assert rel_err(marked(xh[:1]).cpu().numpy(), want[0][:1].double().cpu().numpy()) <= 3e-3
