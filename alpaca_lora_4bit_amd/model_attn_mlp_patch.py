@@ -644,11 +644,22 @@ def _keep_8_bits(mlp):
     return True
 
 
+def _keep_16_bits(mlp):
+    """Takes a block's mark off, and a forward that is there for it alone; whether it had one."""
+    d = mlp.__dict__
+    if d.pop('_q4_act_bits', None) is None:
+        return False
+    if getattr(d.get('forward'), '__func__', None) is _mlp_gated_forward:
+        for name in ('forward', '_q4_mlp_forward', '_q4_mlp_gated'):
+            del d[name]
+    return True
+
+
 def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step=True, act_bits=16):
     """One launch for gate_proj / up_proj of every MLP block (model_attn_mlp_patch.py:163-247; the reference's Triton
     fused-MLP kernel is replaced by one launch over both projections followed by the block's own activation).  In place
     by default; then, with `fuse_decode_step` and a SiLU block of three 4-bit layers of the same group size, the block's
-    forward runs the whole decode step (gate, up, silu(gate) * up, down) as one launch or two.  Returns the number of blocks grouped.
+    forward runs the whole decode step (gate, up, silu(gate) * up, down) as one launch or two.  Returns the number of blocks grouped (or given back 16 bits).
 
     `act_bits=8` (in place and with `fuse_decode_step` only): SiLU blocks of three 4-bit layers, of any group sizes, whose forward is known to be that
     expression keep the outputs of gate and up for their backward pass in 8 bits; second derivatives through them are refused.  Returns the number of blocks
@@ -663,6 +674,7 @@ def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step
     count, as_they_are = 0, []
     for path, m in list(model.named_modules()):
         if all(hasattr(m, n) for n in names + ("down_proj",)):
+            given_back = act_bits == 16 and _keep_16_bits(m)
             if concatenate:
                 count += bool(_fuse_children(m, names, "gate_up_proj"))
                 continue
@@ -679,7 +691,7 @@ def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step
                 if not kept:
                     as_they_are.append(path or type(m).__name__)
             else:
-                count += group is not None
+                count += group is not None or given_back
     if as_they_are:
         warnings.warn(f"{len(as_they_are)} MLP blocks keep their activations as they are (not three 4-bit layers, another activation than SiLU, or a forward of "
                       f"their own): {', '.join(as_they_are)}")

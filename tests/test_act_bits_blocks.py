@@ -73,3 +73,13 @@ def test_without_the_option_nothing_has_changed():
     model = nn.ModuleList([Block(128), Block(-1), Block(128, act=nn.GELU())])
     assert make_fused_mlp(model) == 3 and make_fused_mlp(model) == 0
     assert ["forward" in b.__dict__ for b in model] == [True, False, False]
+
+
+def test_16_bits_can_be_asked_for_again():
+    from alpaca_lora_4bit_amd import model_attn_mlp_patch as patch
+    model = nn.ModuleList([Block(128), Block(-1)])
+    assert patch.make_fused_mlp(model, act_bits=8) == 2
+    assert patch.make_fused_mlp(model, act_bits=16) == 2 and not any(_marked(b) for b in model)
+    assert model[0].forward.__func__ is patch._mlp_decode_forward and "forward" not in model[1].__dict__          # as without the option
+    assert patch.make_fused_mlp(model) == 0
+    assert patch.make_fused_mlp(model, act_bits=8) == 2 and all(_marked(b) for b in model)
