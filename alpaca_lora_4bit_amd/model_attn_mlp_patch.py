@@ -544,12 +544,14 @@ def _gated_rows_forward(mlp, x):
     11008: 24 / 37 as five elementwise kernels, 16 / 24 as two).  Only for forwards known to be this expression."""
     from . import quant_hip
     gate, up = mlp.gate_proj(x), mlp.up_proj(x)
+    if mlp.__dict__.get('_q4_act_bits') == 8:                # the same product with and without gradients: a checkpointed block runs both ways
+        train = torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad)
+        if quant_hip.silu_mul_act8_takes(gate, up):
+            return mlp.down_proj(_SiluMulAct8.apply(gate, up) if train else quant_hip.silu_mul_act8(gate, up, keep=False)[0])
+        if train:
+            warnings.warn(f"an MLP block that is to keep 8 bits has gate and up of {gate.dtype} and {up.dtype}; they are kept as they are")
     if not quant_hip.silu_mul_takes(gate, up):
         return mlp.down_proj(mlp.act_fn(gate) * up)
-    if mlp.__dict__.get('_q4_act_bits') == 8:                # the same product with and without gradients: a checkpointed block runs both ways
-        if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
-            return mlp.down_proj(_SiluMulAct8.apply(gate, up))
-        return mlp.down_proj(quant_hip.silu_mul_act8(gate, up, keep=False)[0])
     return mlp.down_proj(_SiluMul.apply(gate, up) if torch.is_grad_enabled() else quant_hip.silu_mul(gate, up))
 
 
@@ -663,7 +665,7 @@ def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step
 
     `act_bits=8` (in place and with `fuse_decode_step` only): SiLU blocks of three 4-bit layers, of any group sizes, whose forward is known to be that
     expression keep the outputs of gate and up for their backward pass in 8 bits; second derivatives through them are refused.  Returns the number of blocks
-    that do; the others, which keep their operands as they are, are named in a warning."""
+    that do; the others, which keep their operands as they are, are named in a warning, as is a block whose gate and up come out as neither float16 nor bfloat16 when it runs."""
     if is_v1_model:
         raise NotImplementedError("v1 (fp zeros) layers are not fused")
     if act_bits not in (8, 16):

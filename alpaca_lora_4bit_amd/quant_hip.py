@@ -1104,6 +1104,12 @@ def silu_mul_act8(gate, up, keep=True):
     return _training().silu_mul_act8(gate, up, bool(keep))
 
 
+def silu_mul_act8_takes(gate, up):
+    """Whether `silu_mul_act8` takes these tensors (plain float16 or bfloat16 CUDA tensors of one shape, however they lie)."""
+    return (_host is not None and type(gate) is torch.Tensor and type(up) is torch.Tensor and gate.is_cuda and gate.device == up.device
+            and gate.dtype == up.dtype and gate.dtype in (torch.float16, torch.bfloat16) and gate.shape == up.shape and gate.numel() < MAX_SILU_MUL)
+
+
 def silu_mul_act8_bwd(dout, kept):
     """(dgate, dup) of silu(gate) * up in dout's type (fp16 or bf16) and shape, at the values that `kept` holds."""
     return _training().silu_mul_act8_bwd(dout, kept)

@@ -75,3 +75,51 @@ def test_a_block_keeps_8_bits_whatever_its_groups(oracle, monkeypatch, groupsize
         kept.clear()
         assert marked(xh[:1]).shape == (1, H) and marked(xh[:12]).shape == (12, H)
         assert rel_err(marked(xh[:1]).cpu().numpy(), want[0][:1].double().cpu().numpy()) <= 3e-3
+
+
+def _then(block, change):
+    """gate's and up's outputs go through `change`."""
+    for lin in (block.gate_proj, block.up_proj):
+        lin.forward = lambda x, own=lin.forward: change(own(x))
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "columns"])
+def test_operands_of_bfloat16_and_cut_out_of_others_are_kept_in_8_bits(oracle, monkeypatch, kind):
+    """Layers whose outputs are bfloat16, or columns of a wider tensor: the block's gradient is that of the operators by themselves."""
+    from alpaca_lora_4bit_amd import quant_hip
+    from alpaca_lora_4bit_amd.model_attn_mlp_patch import make_fused_mlp
+    block = _block(oracle, 128)
+    _then(block, lambda y: y.bfloat16() if kind == "bfloat16" else torch.cat([y, y], -1)[..., :I])
+    down = block.down_proj.forward
+    block.down_proj.forward = lambda act: down(act.half())
+    assert make_fused_mlp(block, act_bits=8) == 1
+    kept = _counted(monkeypatch, "silu_mul_act8")
+    x = _x(oracle, 200).requires_grad_(True)
+    dy = _x(oracle, 200, 5)
+    y = block(x)
+    assert kept == [(200, I)]
+    (got,) = torch.autograd.grad(y, x, dy.to(y.dtype))
+    gate, up = block.gate_proj(x), block.up_proj(x)
+    out, held = quant_hip.silu_mul_act8(gate.detach(), up.detach())
+    act = out.requires_grad_(True)
+    again = block.down_proj(act)
+    assert torch.equal(y, again)
+    (dact,) = torch.autograd.grad(again, act, dy.to(y.dtype))
+    (want,) = torch.autograd.grad([gate, up], x, list(quant_hip.silu_mul_act8_bwd(dact, held)))
+    assert torch.equal(got, want)
+    kept.clear()
+    with torch.no_grad():
+        assert torch.equal(block(x), y) and kept == [None]
+
+
+def test_operands_of_float32_are_kept_as_they_are_and_said_so(oracle, monkeypatch):
+    from alpaca_lora_4bit_amd.model_attn_mlp_patch import make_fused_mlp
+    block = _block(oracle, 128)
+    _then(block, torch.Tensor.float)
+    assert make_fused_mlp(block, act_bits=8) == 1
+    kept = _counted(monkeypatch, "silu_mul_act8")
+    x = _x(oracle, 200).requires_grad_(True)
+    with pytest.warns(UserWarning, match="float32"), torch.amp.autocast("cuda", dtype=torch.float16):
+        y = block(x)
+    y.float().sum().backward()
+    assert not kept and torch.isfinite(x.grad).all()
