@@ -586,12 +586,13 @@ def _adapters_off(layer):
 
 def _mlp_decode_forward(mlp, x):
     """LlamaMLP.forward with the decode step (up to 16 rows, no grad, fp16) as one launch (quant_hip.mlp_decode: gate, up,
-    silu(gate) * up and down) or two (quant_hip.mlp_rows); everything else goes to the block's own forward.  What the step
+    silu(gate) * up and down) or two (quant_hip.mlp_rows); everything else goes to the block's own forward, and all of a block that
+    keeps 8 bits: the step rounds gate, up and silu(gate) to fp16 on the way, its product with gradients does not.  What the step
     needs of the three layers is looked up once and kept while their buffers, adapters and bias switches stay the same objects / values."""
     quant_hip = matmul_utils_4bit.quant_hip
     d = mlp.__dict__
     if (not torch.is_grad_enabled() and x.dtype == torch.float16 and x.is_cuda and autograd_4bit.backend == 'cuda'
-            and matmul_utils_4bit.use_new and matmul_utils_4bit.auto_switch):
+            and matmul_utils_4bit.use_new and matmul_utils_4bit.auto_switch and d.get('_q4_act_bits') != 8):
         cached = d.get('_q4_mlp_args')
         mods = mlp._modules
         gate, up, down = mods['gate_proj'], mods['up_proj'], mods['down_proj']
@@ -664,7 +665,8 @@ def make_fused_mlp(model, is_v1_model=False, concatenate=False, fuse_decode_step
     forward runs the whole decode step (gate, up, silu(gate) * up, down) as one launch or two.  Returns the number of blocks grouped (or given back 16 bits).
 
     `act_bits=8` (in place and with `fuse_decode_step` only): SiLU blocks of three 4-bit layers, of any group sizes, whose forward is known to be that
-    expression keep the outputs of gate and up for their backward pass in 8 bits; second derivatives through them are refused.  Returns the number of blocks
+    expression keep the outputs of gate and up for their backward pass in 8 bits; second derivatives through them are refused, and they run without the
+    one-launch decode step until `act_bits=16` is asked for.  Returns the number of blocks
     that do; the others, which keep their operands as they are, are named in a warning, as is a block whose gate and up come out as neither float16 nor bfloat16 when it runs."""
     if is_v1_model:
         raise NotImplementedError("v1 (fp zeros) layers are not fused")

@@ -123,3 +123,35 @@ def test_operands_of_float32_are_kept_as_they_are_and_said_so(oracle, monkeypatc
         y = block(x)
     y.float().sum().backward()
     assert not kept and torch.isfinite(x.grad).all()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 12])
+@pytest.mark.parametrize("groupsize", [-1, 128])
+def test_a_few_rows_take_the_same_product_with_and_without_gradients(oracle, monkeypatch, rows, groupsize):
+    """The policy's pass runs with gradients, the reference's without: gate's and up's product is the same at the sizes of the one-launch decode step too."""
+    from conftest import rel_err
+    from alpaca_lora_4bit_amd import quant_hip
+    from alpaca_lora_4bit_amd.model_attn_mlp_patch import make_fused_mlp
+    block = _block(oracle, groupsize)
+    make_fused_mlp(block, act_bits=8)
+    kept, products = _counted(monkeypatch, "silu_mul_act8"), []
+    block.down_proj.register_forward_pre_hook(lambda m, args: products.append(args[0].detach()))
+    x = _x(oracle, rows)
+    for training in (True, False):
+        block.train(training)
+        kept.clear(), products.clear()
+        with torch.amp.autocast("cuda", dtype=torch.float16):
+            y = block(x.clone().requires_grad_(True))
+        with torch.no_grad():
+            again = block(x)
+        assert kept == [(rows, I), None]
+        gate, up = block.gate_proj(x), block.up_proj(x)
+        want = quant_hip.silu_mul_act8(gate.detach(), up.detach(), keep=False)[0]
+        # sums over 256 products in another order: gate and up a step (2^-10) apart at most, and the product half a step more
+        assert rel_err(products[1].cpu().numpy(), want.double().cpu().numpy()) <= 3e-3 and rel_err(products[0].cpu().numpy(), want.double().cpu().numpy()) <= 3e-3
+        assert rel_err(again.cpu().numpy(), y.detach().double().cpu().numpy()) <= 3e-3
+    make_fused_mlp(block, act_bits=16)
+    kept.clear()
+    block.down_proj._forward_pre_hooks.clear()
+    with torch.no_grad():
+        assert rel_err(block(x).cpu().numpy(), y.detach().double().cpu().numpy()) <= 3e-3 and not kept
