@@ -35,13 +35,18 @@ def preference_loss(logits, labels, ref_logps, beta=0.1, label_smoothing=0.0):
 
 @contextlib.contextmanager
 def adapters_off(model):
-    """Within it the model computes without its LoRA adapters (Linear4bitLt's, and those of peft's own layers beside them); each layer gets its own
-    state back afterwards."""
+    """Within it the model computes without its LoRA adapters (Linear4bitLt's, and those of peft's own layers beside them) and as in evaluation: with dropout
+    of its own every pass of a reference would be another one.  Each layer gets its own state back afterwards, each module its own mode."""
     layers = [(m, m.disable_adapters) for m in model.modules() if hasattr(m, "lora_A") and hasattr(m, "enable_adapters")]
+    training = [m for m in model.modules() if m.training]
     try:
+        for m in training:
+            m.training = False
         for layer, _ in layers:
             layer.enable_adapters(False)
         yield model
     finally:
         for layer, off in layers:
             layer.enable_adapters(not off)
+        for m in training:
+            m.training = True

@@ -1,0 +1,34 @@
+"""The pass of the reference model: the model without its adapters, as in evaluation, and everything as it was afterwards (CPU)."""
+import pytest
+import torch
+import torch.nn as nn
+
+
+def _lora(**kw):
+    from alpaca_lora_4bit_amd.models import Linear4bitLt
+    return Linear4bitLt("default", 128, 128, 128, False, r=8, lora_alpha=16, **kw)
+
+
+def test_the_reference_has_no_dropout():
+    """Dropout of the host model would make each pass of the reference another one."""
+    from alpaca_lora_4bit_amd.preference import adapters_off
+
+    class Host(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.q_proj, self.drop, self.still = _lora(lora_dropout=0.1), nn.Dropout(0.5), nn.Dropout(0.5)
+
+        def forward(self, x):
+            return nn.functional.dropout(self.drop(x), 0.5, self.training)
+    model = Host().train()
+    model.still.eval()
+    modes = [m.training for m in model.modules()]
+    x = torch.ones(4096)
+    with pytest.raises(KeyError), adapters_off(model) as same:
+        assert same is model and torch.equal(model(x), x) and not any(m.training for m in model.modules())
+        raise KeyError
+    assert [m.training for m in model.modules()] == modes and not model.still.training and not torch.equal(model(x), x)
+    model.eval()
+    with adapters_off(model):
+        pass
+    assert not any(m.training for m in model.modules())
