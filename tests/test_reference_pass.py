@@ -32,3 +32,14 @@ def test_the_reference_has_no_dropout():
     with adapters_off(model):
         pass
     assert not any(m.training for m in model.modules())
+
+
+def test_a_model_without_adapters_is_refused():
+    """Policy and reference would be one and the same, and the loss log 2 for good."""
+    from alpaca_lora_4bit_amd.preference import adapters_off
+    for model in (nn.Sequential(nn.Linear(3, 3)), nn.Linear(3, 3)):
+        with pytest.raises(ValueError, match="adapter"), adapters_off(model):
+            raise KeyError
+    layer = _lora()                                            # the model may be one layer
+    with adapters_off(layer):
+        assert layer.disable_adapters
