@@ -36,12 +36,13 @@ def preference_loss(logits, labels, ref_logps, beta=0.1, label_smoothing=0.0):
 @contextlib.contextmanager
 def adapters_off(model):
     """Within it the model computes without its LoRA adapters (Linear4bitLt's, and those of peft's own layers beside them) and as in evaluation: with dropout
-    of its own every pass of a reference would be another one.  Each layer gets its own state back afterwards, each module its own mode.
-    A model without adapters is refused."""
+    of its own every pass of a reference would be another one.  Each layer gets its own state back afterwards, each module its own mode and each parameter of a layer its own
+    requires_grad.  A model without adapters is refused."""
     layers = [(m, m.disable_adapters) for m in model.modules() if hasattr(m, "lora_A") and hasattr(m, "enable_adapters")]
     if not layers:
         raise ValueError("the model has no LoRA adapters to switch off: it would be its own reference")
     training = [m for m in model.modules() if m.training]
+    trained = [(p, p.requires_grad) for layer, _ in layers for p in layer.parameters()]      # peft's own switch sets it too
     try:
         for m in training:
             m.training = False
@@ -51,5 +52,7 @@ def adapters_off(model):
     finally:
         for layer, off in layers:
             layer.enable_adapters(not off)
+        for p, wanted in trained:
+            p.requires_grad_(wanted)
         for m in training:
             m.training = True

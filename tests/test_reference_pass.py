@@ -43,3 +43,32 @@ def test_a_model_without_adapters_is_refused():
     layer = _lora()                                            # the model may be one layer
     with adapters_off(layer):
         assert layer.disable_adapters
+
+
+def test_frozen_adapters_stay_frozen():
+    """Layers whose switch also decides what is trained: off freezes the adapters, on makes the active ones trainable."""
+    from alpaca_lora_4bit_amd.preference import adapters_off
+
+    class Switched(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.lora_A, self.lora_B = nn.ModuleDict({"a": nn.Linear(4, 2), "b": nn.Linear(4, 2)}), nn.ModuleDict({"a": nn.Linear(2, 4), "b": nn.Linear(2, 4)})
+            self.disable_adapters = False
+
+        def enable_adapters(self, enabled):
+            self.disable_adapters = not enabled
+            for part in (self.lora_A, self.lora_B):
+                for name, layer in part.items():
+                    layer.requires_grad_(enabled and name == "a")
+    frozen, other, trained = Switched(), Switched(), Switched()
+    for p in frozen.parameters():
+        p.requires_grad_(False)
+    other.enable_adapters(False)
+    other.lora_B["b"].weight.requires_grad_(True)
+    model = nn.ModuleList([frozen, other, trained])
+    before = [p.requires_grad for p in model.parameters()]
+    with pytest.raises(KeyError), adapters_off(model):
+        assert all(m.disable_adapters for m in model)
+        raise KeyError
+    assert [p.requires_grad for p in model.parameters()] == before
+    assert [m.disable_adapters for m in model] == [False, True, False]
