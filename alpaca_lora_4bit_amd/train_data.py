@@ -216,24 +216,31 @@ class TrainPreference(ATrainData):
     def tokenize(self, prompt: str, use_eos_token=True, **kwargs) -> Dict[str, Any]:
         pass                                       # unused: rows are built by tokenize_pair
 
-    def _ids(self, text, room, first=False):
+    def _ids(self, text, room=None, first=False):
         """Ids of `text`, at most `room`; without BOS unless it comes `first`."""
         ids = list(self.tokenizer(text)["input_ids"])
         if not first and ids and ids[0] == self.tokenizer.bos_token_id:
             ids = ids[1:]
-        return ids[:max(room, 0)]
+        return ids if room is None else ids[:max(room, 0)]
+
+    def _ids_behind(self, lead, text):
+        """Ids of `text` as they are behind `lead` (tokenizers mark the beginning of a text, and a word behind a line's end is another one)."""
+        if not lead:
+            return self._ids(text)
+        before, both = self._ids(lead), self._ids(lead + text)
+        return both[len(before):] if both[:len(before)] == before else self._ids(text)
 
     def tokenize_pair(self, record, use_eos_token=True):
         tok, window = self.tokenizer, self.cutoff_len
-        if record.get("prompt") is not None:
-            prompt = record["prompt"]
-        else:                                      # the template of the Alpaca records, up to where the answer begins
+        if record.get("prompt") is not None:       # prompt, newline, answer, each by itself, as in a GPT4All record
+            head, lead = self._ids(record["prompt"], window // 2, first=True), ""
+            head += self._ids("\n", window - len(head))
+        else:                                      # the template of the Alpaca records, up to where the answer begins, and the answer as it follows there
             prompt = TrainSAD.generate_prompt(self, {**{k: v for k, v in record.items() if k in ("instruction", "input") and v is not None}, "output": ""})
-        head = self._ids(prompt, window // 2, first=True)
-        head += self._ids("\n", window - len(head))
+            head, lead = self._ids(prompt, window // 2, first=True), prompt[prompt.rindex("\n\n### Response:"):]
         sample = {}
         for name in ("chosen", "rejected"):
-            answer = self._ids(record[name], window - len(head))
+            answer = self._ids_behind(lead, record[name])[:max(window - len(head), 0)]
             if use_eos_token and len(head) + len(answer) < window:         # a truncated answer gets no EOS
                 answer = answer + [tok.eos_token_id]
             sample[name + "_ids"] = head + answer
