@@ -15,7 +15,8 @@ Sample construction follows the reference:
 * GPT4All records (`:254-330`): prompt (at most half the window), newline, response without BOS, EOS when it fits;
   labels are -100 over prompt, newline and padding.
 * preference records (no counterpart in the reference): a prompt and two answers, "chosen" and "rejected"; each answer becomes a sample like a
-  GPT4All record's, unpadded, and `collate_pairs` puts the chosen ones of a batch before the rejected ones.
+  GPT4All record's, or an Alpaca record's where there is an instruction in place of the prompt (cut to half the window it keeps its
+  last line, where the answer begins), unpadded, and `collate_pairs` puts the chosen ones of a batch before the rejected ones.
 """
 import os
 from abc import ABC, abstractmethod
@@ -207,6 +208,14 @@ class TrainGPT4All(ATrainData):
         self.train_data = encode(records)
 
 
+def _same_at_the_end(a, b):
+    """How many values two lists have in common at their ends."""
+    count = 0
+    while count < min(len(a), len(b)) and a[-1 - count] == b[-1 - count]:
+        count += 1
+    return count
+
+
 class TrainPreference(ATrainData):
     """Records of a prompt, the answer to prefer to it and the one to reject: "prompt" (or Alpaca's "instruction" and "input"), "chosen", "rejected"."""
 
@@ -237,7 +246,11 @@ class TrainPreference(ATrainData):
             head += self._ids("\n", window - len(head))
         else:                                      # the template of the Alpaca records, up to where the answer begins, and the answer as it follows there
             prompt = TrainSAD.generate_prompt(self, {**{k: v for k, v in record.items() if k in ("instruction", "input") and v is not None}, "output": ""})
-            head, lead = self._ids(prompt, window // 2, first=True), prompt[prompt.rindex("\n\n### Response:"):]
+            lead = prompt[prompt.rindex("\n\n### Response:"):]
+            head = self._ids(prompt, first=True)
+            if len(head) > window // 2:            # its last line stays, and BOS; what is cut off is the end of the request
+                last = min(_same_at_the_end(head, self._ids(lead)), max(window // 2 - 1, 0))
+                head = head[:window // 2 - last] + head[len(head) - last:]
         sample = {}
         for name in ("chosen", "rejected"):
             answer = self._ids_behind(lead, record[name])[:max(window - len(head), 0)]
