@@ -6,6 +6,7 @@ again by the world size under DDP (`:85-86`); dropout forced to 0 with gradient 
 `val_set_size` above 1 is a row count, otherwise a fraction (`:71`); `WORLD_SIZE` / `LOCAL_RANK` from the
 environment decide `ddp` and `device_map` (`:81-84`).
 """
+import math
 import os
 
 _PLAIN_FIELDS = (
@@ -27,6 +28,21 @@ _SUMMARY = (
 )
 
 
+def check_beta(value):
+    """What the preference loss takes for beta, as a float."""
+    value = float(value)
+    if not 0.0 < value < math.inf:
+        raise ValueError(f"beta must be positive and finite, not {value}")
+    return value
+
+
+def check_label_smoothing(value):
+    value = float(value)
+    if not 0.0 <= value <= 0.5:
+        raise ValueError(f"label_smoothing must be in [0, 0.5], not {value}")
+    return value
+
+
 class Finetune4bConfig:
     """Config holder for 4-bit LLaMA LoRA finetuning; keyword arguments as in the reference (`:5-20`) and three of its own: `act_bits` (8: checkpoints and
     the MLP blocks' activations in 8 bits), `beta` and `label_smoothing` (preference loss)."""
@@ -37,6 +53,9 @@ class Finetune4bConfig:
                  save_total_limit, logging_steps, checkpoint, skip, verbose, txt_row_thd, use_eos_token, groupsize,
                  v1, local_rank, flash_attention, xformers, backend, act_bits=16, beta=0.1, label_smoothing=0.0):
         given = locals()
+        if act_bits not in (8, 16):
+            raise ValueError(f"act_bits must be 8 or 16, not {act_bits}")
+        check_beta(beta), check_label_smoothing(label_smoothing)
         for name in _PLAIN_FIELDS:
             setattr(self, name, given[name])
         self.lora_dropout = 0 if gradient_checkpointing else lora_dropout

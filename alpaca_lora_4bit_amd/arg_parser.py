@@ -9,7 +9,17 @@ Options that the reference lacks (`--act_bits`, `--beta`, `--label_smoothing`) a
 import argparse
 import os
 
-from .Finetune4bConfig import Finetune4bConfig
+from .Finetune4bConfig import Finetune4bConfig, check_beta, check_label_smoothing
+
+
+def _checked(check):
+    def value(text):
+        try:
+            return check(text)
+        except ValueError as e:
+            raise argparse.ArgumentTypeError(str(e)) from None
+    return value
+
 
 # (group, flags, argparse keywords); help texts are generated from the defaults
 _CONFIG, _TRAINING = "config", "training"
@@ -50,8 +60,8 @@ _OPTIONS = (
     (_TRAINING, ("--backend",), dict(default="cuda", type=str, help="Kernel backend name: cuda or triton")),
     (_TRAINING, ("--act_bits",), dict(default=argparse.SUPPRESS, type=int, choices=[8, 16], help="8: checkpoints and the MLP blocks' activations are kept in 8 bits "
                                       "for the backward pass. Default: 16, as they are")),
-    (_TRAINING, ("--beta",), dict(default=argparse.SUPPRESS, type=float, help="Preference loss: factor of the log ratios. Default: 0.1")),
-    (_TRAINING, ("--label_smoothing",), dict(default=argparse.SUPPRESS, type=float, help="Preference loss: share of pairs taken to be the wrong way round. Default: 0")),
+    (_TRAINING, ("--beta",), dict(default=argparse.SUPPRESS, type=_checked(check_beta), help="Preference loss: factor of the log ratios. Default: 0.1")),
+    (_TRAINING, ("--label_smoothing",), dict(default=argparse.SUPPRESS, type=_checked(check_label_smoothing), help="Preference loss: share of pairs taken to be the wrong way round. Default: 0")),
 )
 
 # argparse destination -> Finetune4bConfig keyword where the two differ
