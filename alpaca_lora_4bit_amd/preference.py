@@ -13,7 +13,9 @@ from . import quant_hip
 
 def shifted_labels(labels):
     """labels [B, S] of the tokens themselves -> [B, S] of the tokens that the logits at each place predict: one place to the left, the last place none."""
-    return torch.nn.functional.pad(labels[..., 1:], (0, 1), value=-100)
+    moved = torch.full_like(labels, -100, memory_format=torch.contiguous_format)
+    moved[..., :-1] = labels[..., 1:]
+    return moved
 
 
 def token_logps(logits, labels):

@@ -72,3 +72,13 @@ def test_frozen_adapters_stay_frozen():
         raise KeyError
     assert [p.requires_grad for p in model.parameters()] == before
     assert [m.disable_adapters for m in model] == [False, True, False]
+
+
+def test_labels_of_no_place_stay_of_no_place():
+    from alpaca_lora_4bit_amd.preference import shifted_labels
+    for shape in ((3, 0), (0, 4), (2, 0, 0), (0,)):
+        moved = shifted_labels(torch.zeros(shape, dtype=torch.long))
+        assert moved.shape == shape and moved.dtype == torch.long
+    base = torch.arange(24).view(2, 3, 4)
+    assert shifted_labels(base).tolist() == [[[*row[1:], -100] for row in part] for part in base.tolist()]
+    assert torch.equal(shifted_labels(base.transpose(1, 2))[..., :2], base.transpose(1, 2)[..., 1:])
