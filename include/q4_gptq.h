@@ -453,8 +453,8 @@ Q4_API int q4_token_logps_bwd(const void *logits, int type, long long sb, long l
                        int per, const float *factor, void *dlogits, void *stream);
 /* P pairs in logits [2P, S, V]: sequences p (preferred) and p + P (rejected).  r_b = sum over the tokens (labels as above) of log-probability - ref, ref fp32
  * [2P, S], not used where the label is no token; z_p = beta * (r_p - r_{p+P}); loss = mean over p of -(1 - smoothing) log sigmoid(z_p) - smoothing
- * log sigmoid(-z_p); rewards fp32 [2P] = beta * r; coef fp32 [2P] = dloss / dr, what q4_token_logps_bwd takes with per = S, stats as there.  Log-probabilities,
- * their sums (in a fixed order) and the loss in fp64.  beta > 0 and finite, 0 <= smoothing <= 0.5.  `workspace`: the bytes that the query gives, 8-byte aligned,
+ * log sigmoid(-z_p); rewards fp32 [2P] = beta * r; coef fp32 [2P] = dloss / dr, what q4_token_logps_bwd takes with per = S, stats as there.  Exponentials
+ * in fp32, their sums, the log-probabilities, the answers' sums (all in a fixed order) and the loss in fp64.  beta > 0 and finite, 0 <= smoothing <= 0.5.  `workspace`: the bytes that the query gives, 8-byte aligned,
  * contents irrelevant. */
 Q4_API size_t q4_preference_loss_workspace_bytes(int P, int S);
 Q4_API int q4_preference_loss(const void *logits, int type, long long sb, long long st, int P, int S, int V, const long long *labels, const float *ref, double beta,
