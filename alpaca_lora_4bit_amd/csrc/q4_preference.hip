@@ -5,7 +5,7 @@
 // HBM-bound: one pass over a row's logits, backward one pass more from the L that forward left (an answer's factor c needs all of its tokens first).
 // Rows whose label is not one of the V words are no tokens of an answer (a prompt, padding): they are not read, and their gradient is zero.
 // Exponentials in fp32, their sums and what follows in fp64: a log ratio is the small difference of sums of some hundred log-probabilities, and an
-// error in one direction grows with the answer (measured over answers of 2048 tokens: 1.5e-9 a token at most).  us and TB/s moved, 16 pairs of 1024 places of 32000
+// error in one direction grows with the answer (over answers of 2048 tokens 1.1e-9 a token at most).  us and TB/s moved, 16 pairs of 1024 places of 32000
 // words in fp16 of which 17370 are tokens: forward 186 (6.0), log ratios and loss 10, backward 527 (6.1); a large copy reaches 5.15.
 #include "q4_common.hpp"
 #include "q4_gptq.h"
@@ -14,7 +14,9 @@
 namespace q4 {
 
 constexpr float kLog2eHi = 0x1.715476p+0f, kLog2eLo = 0x1.4ae0c0p-26f;       // log2(e) in two parts
-constexpr double kExpShort = 3e-9;                                           // v_exp_f32 is short by so much of itself on average (measured: sum of 4 million)
+// v_exp_f32 is short by so much of itself on average: 1.24e-9 for arguments of 1 and more, 3.42e-9 for -1 and less, over all fp32 numbers of each power of
+// two's range up to 128; what is left, 1.1e-9, is that of a row whose words all lie on one side of its label.
+constexpr double kExpShort = 2.33e-9;
 
 // exp(d).  With one fp32 factor log2(e) every exponent is short by 1.3e-8 of itself: all in one direction, which a log ratio over a
 // long answer adds up.
@@ -197,6 +199,8 @@ __global__ __launch_bounds__(THREADS) void token_logps_bwd_kernel(LogitsView a, 
         const T* x = row_of<T>(a, row);
         const float2 st = stats[row];
         const float c = (factor ? *factor : 1.f) * coef[row / per];
+        // In fp32: the distance to L is off by half a unit of itself, its exponent by 1.3e-8 (one log2(e)), together 1e-6 of a probability of e^-16 and less of larger
+        // ones: below the rounding to 16 bits, and in fp32 what softmax's own gradient has; no sum of these needs more.
         auto share = [&](T v) { return (T)(-c * __expf(((float)v - st.x) - st.y)); };
         // the label's own gradient c (1 - p), formed without that difference
         auto own = [&](T v) { return (T)(-c * expm1f(((float)v - st.x) - st.y)); };
