@@ -983,7 +983,7 @@ at::Tensor act8_unpack(const at::Tensor& codes, const at::Tensor& scales, at::Sc
 }
 
 // What a gated activation keeps, in one piece of memory: the codes of gate and of up, then their scales, each from a 16-byte boundary on.  One
-// tensor is allocated, saved and checked where four would be (a short sample, forward and backward: 12.7 -> 9.8 us).
+// tensor is allocated, saved and checked where four would be (a short sample, forward and backward: 12.2 -> 10.2 us).
 struct Kept {
     q4_act8_t gate, up;
     static int64_t codes(int64_t n) { return (n + 15) / 16 * 16; }

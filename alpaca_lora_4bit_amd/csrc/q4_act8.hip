@@ -6,8 +6,9 @@
 //
 // HBM-bound: a lane takes 8 neighbours (one 16-byte load of 16-bit values), a block is the four lanes of a quad, its maximum two lane exchanges; one such
 // piece a lane and 256 threads a workgroup (512 and 1024: the same or slower; codes stored past the caches: forward 19.3 -> 18.1 us at 1024 x 11008, but what
-// reads them soon then waits for HBM, 2 us).  us and TB/s moved, operands from HBM: 16384 x 5120 fp32 packed 73 (5.8), read back 77 (5.5); 8192 x 13824
-// bfloat16 through silu(gate) * up 160 (5.7), backward 159 (5.8); a large copy reaches 5.15.
+// reads them soon then waits for HBM, 2 us).  us and TB/s moved, operands from HBM: 16384 x 5120 fp32 packed 72 (5.8), read back 74 (5.6), call after call;
+// packed and read back in turn 162 (5.1: each finds the caches full of what the other wrote).  8192 x 13824 bfloat16 through silu(gate) * up 160 (5.6), backward 158 (5.7);
+// a large copy reaches 5.13.
 #include <type_traits>
 #include "q4_act8.hpp"
 

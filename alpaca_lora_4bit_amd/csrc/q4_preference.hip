@@ -117,8 +117,8 @@ __device__ __forceinline__ double group_sum(double v, double* lds) {
 }
 
 // A row's sum of exp(x - at), at = the label's own logit: exponents need no maximum first, and what follows is -log(sum).  Where the label's logit is
-// so far below others that this leaves fp32 (by 80 and more), is no number, or the row has an infinity, the row is read again for its maximum and once more
-// for the sum beside it.  `logps` or `wide` (the other is null) takes the log-probability: in fp32 for a caller, in fp64 for the log ratios.
+// so far below others that this leaves fp32 (by 80 and more), or is -infinity, or the row has a NaN or +infinity, the row is read again for its maximum and once more
+// for the sum beside it; -infinity elsewhere is no weight at the first reading.  `logps` or `wide` (the other is null) takes the log-probability: in fp32 for a caller, in fp64 for the log ratios.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_logps_kernel(LogitsView a, const long long* __restrict__ labels, float* __restrict__ logps, double* __restrict__ wide,
                                                               float2* __restrict__ stats) {
@@ -313,10 +313,15 @@ int by_type(int type, F&& launch) {
 
 }  // namespace q4
 
-// Threads of a row's workgroup.  Wavefronts by themselves for rows of up to 4 KB (32768 rows of 640 bytes, forward / backward: 64 threads 15 / 17 us,
-// 256 34 / 39).  Forward 256 with eight loads a thread on their way (32768 rows of 64 KB, 0.55 of them tokens: 190 us, four loads 198), and 512 where there are few
-// rows or long ones (37 rows of 64 KB: 7.6 against 8.5, 2048 of 256 KB 96 against 110; 1024 threads wait for each other: 415 against 190).  Backward, where
-// nothing waits, 1024 for rows of 48 KB and more, its stores past the caches (the same rows: 520 us, through them 587, with 256 threads 622).
+// Threads of a row's workgroup, by the bytes of a row and, forward, how many rows there are (with those that have no label, for labels are device memory).  us, fp16:
+//   64 / 256 threads (a wavefront by itself, or four), up to 4 KB a row.  32768 rows of 2, 4, 8 KB: forward 24 / 62, 31 / 67, 52 / 91, backward 26 / 52, 47 / 64,
+//     94 / 92; 2048 rows of 4 KB 5.1 / 6.5 and 5.5 / 6.4; 256 rows the same.  Forward a wavefront would win beyond 4 KB, where this does not take it.
+//   forward 256 / 512, beyond 512 rows of less than 192 KB.  64 KB a row: 37 rows 5.5 / 5.2, 256 7.4 / 6.6, 512 9.4 / 9.3, 768 13.5 / 13.6, 1024 17.1 / 18.2,
+//     2048 27.4 / 28.1, 32768 of which 0.55 are tokens 190 / 218; 2048 rows of 16 KB 10.2 / 12.1.  1024 and 4096 rows of 128 KB 28.4 / 29.5 and 97 / 93, of 192 KB 40.1 / 41.3
+//     and 144 / 136, of 256 KB 51 / 54 and 186 / 179.  256 with eight loads a thread on their way (four: 198 for 190); 1024 threads wait for each other (415).
+//   backward, where nothing waits, 256 / 1024 past the caches / 1024 through them, up to 48 KB.  16384 rows of 32 KB 189 / 215 / 216, of 48 KB 296 / 263 / 268, of 64 KB 402 /
+//     331 / 339; 1024 rows of 48 KB 21.8 / 20.3 / 22.8, 37 of 64 KB 6.2 / 5.0 / 5.0.  With a kernel behind it that reads the gradient: 1024 rows of 48 KB 35.2 / 37.6 / 36.6,
+//     of 64 KB 46.9 / 47.0 / 45.2, 16384 rows of 64 KB 741 / 671 / 677.
 namespace {
 template <typename F>
 void by_width(bool forward, long rows, long bytes, F&& launch) {
