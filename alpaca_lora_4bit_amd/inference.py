@@ -152,13 +152,13 @@ def _passed_by(module, cls):
     transformers' LLaMA class `cls`.  None where there is no such thing: this package's groups and its wrappers of a forward (autocast,
     checkpointing, the fused MLP step) are known to change nothing here."""
     from .gradient_checkpointing import _ForwardPatch
-    from .model_attn_mlp_patch import _FusedGroup, _MemberGroup, _mlp_decode_forward
+    from .model_attn_mlp_patch import _FusedGroup, _MemberGroup, _mlp_decode_forward, _mlp_gated_forward
     for hooks in (module._forward_hooks, module._forward_pre_hooks, module._backward_hooks, module._backward_pre_hooks):
         if any(not isinstance(getattr(h, "__self__", None), (_FusedGroup, _MemberGroup)) for h in hooks.values()):
             return "a hook"
     own = module.__dict__
     forward = own.get("forward")
-    if "_q4_mlp_forward" in own and getattr(forward, "__func__", None) is _mlp_decode_forward:
+    if "_q4_mlp_forward" in own and getattr(forward, "__func__", None) in (_mlp_decode_forward, _mlp_gated_forward):
         forward = own["_q4_mlp_forward"]
     elif "non_autocast_forward" in own and getattr(forward, "__wrapped__", None) is own["non_autocast_forward"]:
         forward = own["non_autocast_forward"]

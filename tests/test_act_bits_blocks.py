@@ -83,3 +83,22 @@ def test_16_bits_can_be_asked_for_again():
     assert model[0].forward.__func__ is patch._mlp_decode_forward and "forward" not in model[1].__dict__          # as without the option
     assert patch.make_fused_mlp(model) == 0
     assert patch.make_fused_mlp(model, act_bits=8) == 2 and all(_marked(b) for b in model)
+
+
+@pytest.mark.parametrize("groupsize", [-1, 128])
+def test_a_batch_of_requests_takes_marked_blocks_apart(groupsize):
+    """Their forward in place of the block's own changes nothing that a batch would leave out."""
+    from transformers import LlamaConfig, LlamaForCausalLM
+    from alpaca_lora_4bit_amd.autograd_4bit import find_layers, make_quant_for_4bit_autograd
+    from alpaca_lora_4bit_amd.inference import _passed_by
+    from alpaca_lora_4bit_amd.model_attn_mlp_patch import make_fused_mlp
+    model = LlamaForCausalLM(LlamaConfig(vocab_size=97, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=4))
+    layers = find_layers(model)
+    del layers["lm_head"]
+    make_quant_for_4bit_autograd(model, layers, groupsize=groupsize)
+    for bits in (8, 16, 8):
+        assert make_fused_mlp(model, act_bits=bits) == 2
+        assert all(_marked(b.mlp) == (bits == 8) and _passed_by(b.mlp, "LlamaMLP") is None for b in model.model.layers)
+    mlp = model.model.layers[0].mlp
+    mlp.forward = lambda x, inner=mlp.forward: inner(x)
+    assert _passed_by(mlp, "LlamaMLP") == "a replaced forward"
