@@ -127,7 +127,7 @@ def _preference_trainer():
             return (loss, {"rewards": rewards}) if return_outputs else loss
 
         def log(self, logs, *args, **kwargs):
-            """With every line of losses the share of pairs that are the right way round, and by how much."""
+            """With every line of losses the share of this process's pairs that are the right way round, and by how much."""
             for training, key, prefix in ((True, "loss", ""), (False, "eval_loss", "eval_")):
                 if key in logs and self._margins[training]:
                     margins = torch.cat(self._margins[training])

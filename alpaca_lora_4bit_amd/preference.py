@@ -3,6 +3,9 @@ ratios against a reference, sigmoid loss).
 
 The reference trains on next tokens only (finetune.py:126-180 of it).  The model that a pair's log ratios are taken against is the same model
 with its adapters switched off (`adapters_off`), so no second set of weights is needed.
+
+In a captured graph both functions have their forward and backward pass in one capture, on leaves that no living eager graph holds (torch's accumulation of a
+leaf's gradient stays on the stream that it was made on, and a capture that meets another stream ends the process).
 """
 import contextlib
 
