@@ -587,7 +587,7 @@ def _adapters_off(layer):
 def _mlp_decode_forward(mlp, x):
     """LlamaMLP.forward with the decode step (up to 16 rows, no grad, fp16) as one launch (quant_hip.mlp_decode: gate, up,
     silu(gate) * up and down) or two (quant_hip.mlp_rows); everything else goes to the block's own forward, and all of a block that
-    keeps 8 bits: the step rounds gate, up and silu(gate) to fp16 on the way, its product with gradients does not.  What the step
+    keeps 8 bits: the step rounds silu(gate) to fp16 on the way, the block's product with gradients does not.  What the step
     needs of the three layers is looked up once and kept while their buffers, adapters and bias switches stay the same objects / values."""
     quant_hip = matmul_utils_4bit.quant_hip
     d = mlp.__dict__
